@@ -174,6 +174,38 @@ class GGUFModelC(C.Structure):
     ]
 
 
+class PagedTableC(C.Structure):
+    """vireo_paged_table (include/vireo_paged.h)."""
+    _fields_ = [("max_seqs", C.c_int), ("max_blocks", C.c_int), ("n_blocks", C.c_int), ("block_tokens", C.c_int),
+                ("blocks", c_vp), ("len", c_vp), ("free_blocks", c_vp), ("n_free", c_vp)]
+
+
+class PagedCacheC(C.Structure):
+    """vireo_paged_cache (include/vireo_paged.h)."""
+    _fields_ = [("type", C.c_uint32), ("n_blocks", C.c_int), ("block_tokens", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_size", C.c_int), ("k", c_vp), ("v", c_vp), ("means", c_vp)]
+
+
+class PagedRowsC(C.Structure):
+    """vireo_paged_rows (include/vireo_paged.h)."""
+    _fields_ = [
+        ("rows", C.c_int), ("n_heads", C.c_int), ("type", C.c_uint32),
+        ("q", c_vp), ("k", c_vp), ("v", c_vp),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+        ("q_bias", c_vp), ("k_bias", c_vp), ("v_bias", c_vp),
+        ("q_norm", c_vp), ("k_norm", c_vp), ("eps", C.c_float),
+        ("rope", c_vp), ("rotary", C.c_int), ("max_pos", C.c_int),
+        ("positions", c_vp), ("slots", c_vp),
+        ("q_out", c_vp), ("q_out_type", C.c_uint32), ("q_out_stride", C.c_int64),
+    ]
+
+
+class PagedPlanC(C.Structure):
+    """vireo_paged_plan (include/vireo_paged.h)."""
+    _fields_ = [("table", C.POINTER(PagedTableC)), ("ids", c_vp), ("n", C.c_int), ("n_heads", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_size", C.c_int), ("list_blocks", C.c_int), ("mem", c_vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "vireo_hip_init": (C.c_int, [C.c_int]),
@@ -250,6 +282,17 @@ SIGNATURES = {
     "vireo_kv_attend_gqa": (C.c_int, [c_vp, C.c_int, C.c_int, C.c_int, c_vp, c_vp, c_vp]),
     "vireo_kv_stats": (None, [c_vp, C.POINTER(KVStats)]),
     "vireo_kv_destroy": (None, [c_vp]),
+    "vireo_paged_reset": (C.c_int, [C.POINTER(PagedTableC), c_vp]),
+    "vireo_paged_extend": (C.c_int, [C.POINTER(PagedTableC), c_vp, c_vp, C.c_int, C.c_int, c_vp, c_vp, c_vp, c_vp,
+                                     c_vp]),
+    "vireo_paged_truncate": (C.c_int, [C.POINTER(PagedTableC), c_vp, c_vp, C.c_int, c_vp]),
+    "vireo_paged_append": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedRowsC), c_vp]),
+    "vireo_paged_plan_bytes": (C.c_int64, [C.POINTER(PagedPlanC)]),
+    "vireo_paged_plan_update": (C.c_int, [C.POINTER(PagedPlanC), c_vp]),
+    "vireo_paged_attend": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedPlanC), c_vp, C.c_uint32, C.c_int64,
+                                     C.c_float, c_vp, c_vp, C.c_int64, c_vp]),
+    "vireo_paged_select": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedPlanC), c_vp, C.c_uint32, C.c_int64,
+                                     C.c_int, C.c_int, c_vp, c_vp]),
 }
 
 _lib = None

@@ -1,0 +1,137 @@
+// Shared by the paged cache's kernels (API: include/vireo_paged.h): argument
+// checks, the layout of a plan's memory, and 16-bit element types.
+#pragma once
+#include "common.h"
+#include "vireo_paged.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kPagedMaxSeqs = 4096;
+constexpr int kPagedUnit = 128;  // tokens of the unit that a plan splits sequences by
+
+// a pointer that is given and aligned to 16 bytes
+inline bool vh_al16(const void *p) { return p && !(reinterpret_cast<uintptr_t>(p) & 15u); }
+
+inline bool vh_table_ok(const vireo_paged_table *t) {
+    return t && t->max_seqs >= 1 && t->max_seqs <= kPagedMaxSeqs && t->max_blocks >= 1 && t->n_blocks >= 1 &&
+           (t->block_tokens == 16 || t->block_tokens == 32 || t->block_tokens == 64 || t->block_tokens == 128) &&
+           int64_t(t->n_blocks) * t->block_tokens < (int64_t(1) << 31) &&
+           int64_t(t->max_blocks) * t->block_tokens < (int64_t(1) << 31) && t->blocks && t->len && t->free_blocks &&
+           t->n_free;
+}
+
+inline bool vh_cache_ok(const vireo_paged_cache *c) {
+    return c && (c->type == VIREO_PAGED_F16 || c->type == VIREO_PAGED_BF16) && c->n_blocks >= 1 && c->n_kv_heads >= 1 &&
+           c->n_kv_heads <= 65535 &&
+           (c->block_tokens == 16 || c->block_tokens == 32 || c->block_tokens == 64 || c->block_tokens == 128) &&
+           int64_t(c->n_blocks) * c->block_tokens < (int64_t(1) << 31) &&
+           (c->head_size == 64 || c->head_size == 128 || c->head_size == 256) && vh_al16(c->k) && vh_al16(c->v) &&
+           (!c->means || vh_al16(c->means));
+}
+
+// rows of `heads` heads of hs elements of `type`, `stride` elements apart, each 16-byte aligned
+inline bool vh_rows_ok(const void *p, uint32_t type, int64_t stride, int64_t heads, int hs, int64_t rows) {
+    if (!vh_al16(p) || (type != VIREO_PAGED_F32 && type != VIREO_PAGED_F16 && type != VIREO_PAGED_BF16)) return false;
+    const int64_t per16 = type == VIREO_PAGED_F32 ? 4 : 8;
+    return stride % per16 == 0 && (rows <= 1 || stride >= heads * hs) && stride >= 0 && stride < (int64_t(1) << 40);
+}
+
+// ---- a plan's memory ------------------------------------------------------------
+// A batch is cut into items: (sequence, run of kPagedUnit-token units). Items of
+// a sequence are consecutive; first[i] is sequence i's first. Every kv head (and
+// tile of 16 query heads of it) attends each item in one workgroup.
+struct PlanHead {
+    uint32_t tag;  // written by an update of a plan of the same shape (vh_plan_tag)
+    int32_t n_items;
+    int32_t pad[14];
+};
+struct PlanItem {
+    int32_t row;         // of the table
+    int32_t begin, end;  // tokens (of the listed blocks, where the plan has lists)
+    int32_t seq;         // in the batch; bit 31: the sequence's only item
+};
+struct PlanView {
+    PlanHead *head;
+    int32_t *first;   // [n + 1]
+    PlanItem *items;  // [cap]
+    uint32_t *keys;   // [n x n_kv_heads x max_blocks] ordered scores (plans with lists)
+    float2 *ml;       // [cap x n_heads] largest score and sum of weights of each item's partial
+    float *part;      // [cap x n_heads x head_size]
+    int cap;
+    uint32_t tag;
+    int64_t bytes;
+};
+bool vh_plan_ok(const vireo_paged_plan *p);    // its fields but mem
+PlanView vh_plan_view(const vireo_paged_plan *p);
+int vh_plan_head_tiles(const vireo_paged_plan *p);  // tiles of 16 query heads per kv head
+
+// ---- device ---------------------------------------------------------------------
+VH_DEV float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+VH_DEV float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// 16-bit element types by the type number: two packed values <-> floats (rounded to nearest even)
+template <uint32_t T>
+struct El;
+template <>
+struct El<VIREO_PAGED_BF16> {
+    static VH_DEV float2 unpack(uint32_t w) { return make_float2(bf_lo(w), bf_hi(w)); }
+    static VH_DEV uint32_t pack(float a, float b) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, (b2){__bf16(a), __bf16(b)});
+    }
+    static VH_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct El<VIREO_PAGED_F16> {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    static VH_DEV float2 unpack(uint32_t w) {
+        const h2 v = __builtin_bit_cast(h2, w);
+        return make_float2(float(v[0]), float(v[1]));
+    }
+    static VH_DEV uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, (h2){_Float16(a), _Float16(b)});
+    }
+    static VH_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf16x8, a), __builtin_bit_cast(hf16x8, b), c, 0,
+                                                      0, 0);
+    }
+};
+VH_DEV u32x4 ldu4(const void *p) { return *reinterpret_cast<const u32x4 *>(p); }
+// 8 consecutive elements of a type known at run time (the same for the whole launch) as floats
+VH_DEV void ld8(const void *p, uint32_t type, int64_t i, float (&x)[8]) {
+    if (type == VIREO_PAGED_F32) {
+        const f32x4 a = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i)[0];
+        const f32x4 b = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i)[1];
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = a[j], x[4 + j] = b[j];
+        return;
+    }
+    const u32x4 w = ldu4(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2 v = type == VIREO_PAGED_BF16 ? El<VIREO_PAGED_BF16>::unpack(w[j]) : El<VIREO_PAGED_F16>::unpack(w[j]);
+        x[2 * j] = v.x;
+        x[2 * j + 1] = v.y;
+    }
+}
+VH_DEV u32x4 pack8(const float (&x)[8], uint32_t type) {
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        w[j] = type == VIREO_PAGED_BF16 ? El<VIREO_PAGED_BF16>::pack(x[2 * j], x[2 * j + 1])
+                                        : El<VIREO_PAGED_F16>::pack(x[2 * j], x[2 * j + 1]);
+    return w;
+}
+VH_DEV void st8(void *p, uint32_t type, int64_t i, const float (&x)[8]) {
+    if (type == VIREO_PAGED_F32) {
+        f32x4 *d = reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i);
+        d[0] = f32x4{x[0], x[1], x[2], x[3]};
+        d[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + i) = pack8(x, type);
+    }
+}

@@ -1,0 +1,459 @@
+// Attention of one new token per sequence over the paged cache (API:
+// include/vireo_paged.h), split over the sequences' lengths and joined.
+//
+//   out = sum_t e^(s_t - M) v_t / sum_t e^(s_t - M),  s_t = scale q . k_t,  M = max s_t
+//
+// A workgroup takes one item of the plan (a run of one sequence's tokens) and
+// one kv head with up to 16 of its query heads; its four waves take a quarter
+// of the run's 32-token tiles each. Per tile, all in registers:
+//
+//   S^T = K Q^T   v_mfma 16x16x32: rows are 16 tokens, columns the 16 heads, the
+//                 32 a run of head dimensions. Two such products make the tile:
+//                 row r of product u is token 8 (r / 4) + 4 u + r % 4, so the four
+//                 results of a lane from each are its head's scores of tokens
+//                 8 g .. 8 g + 7 (g = lane / 16).
+//   weights       an online softmax: the running maximum over the head's four
+//                 lanes, e^(s - m) in fp32, the sum per lane.
+//   O^T += V^T P^T  rows are 16 dimensions, columns the heads, the 32 the tile's
+//                 tokens: the lane's 8 weights are its operand as they stand, and 16
+//                 consecutive bytes of the cache (8 tokens of a dimension) are V^T's.
+//
+// No weight, key or value passes through LDS or another lane; that is why
+// values lie dimension by dimension in their block. Keys are requested again as
+// soon as the scores are formed and values as soon as they are weighed, so a
+// wave has a tile of 64 hs bytes in flight nearly all the time. Bound by the
+// read of keys and values; the matrix cores take a tenth of that time even with
+// fp32 queries and weights in three parts each.
+//
+// Precision: products of 16-bit parts are exact in the matrix cores and their
+// sums fp32. An fp32 query is the sum of three truncated 16-bit parts (bf16: 24
+// bits; fp16, under a power of two per head: 33 bits), a weight of two (bf16: 16
+// bits, far below the half step 2^-9 of a 16-bit result) or, for fp32 results,
+// three (24 bits) in bf16 and two (22 bits) in fp16. The sum of weights is of
+// the fp32 values. Parts that would be zero get the least value of the query's
+// sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
+//
+// Waves merge through LDS, items in a second launch (merge_kernel) in the
+// items' order: the same bits every time. A sequence of one item is written by
+// the first launch. (A merge by the last workgroup to arrive needs its release
+// fence to write back the L2, which costs more than the launch.)
+#include <hip/hip_runtime.h>
+#include <errno.h>
+#include "paged.h"
+
+namespace {
+
+constexpr float kLowest = -3.4028234663852886e38f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttendArgs {
+    const uint16_t *k, *v;
+    int n_blocks, n_kv, shift;  // block_tokens = 1 << shift
+    const int32_t *table, *len;
+    int max_blocks;
+    const int32_t *lists;  // or null
+    int list_blocks;
+    const void *q;
+    int64_t q_stride;
+    float c;  // scale log2(e): scores in powers of two
+    int n_heads, hpg, tiles;  // query heads, of a kv head, tiles of 16 of those
+    void *out;
+    int64_t out_stride;
+    uint32_t type;  // of q and out
+    PlanHead *head;
+    const PlanItem *items;
+    const int32_t *first;
+    uint32_t tag;
+    float *part;
+    float2 *ml;
+};
+
+// the wave's value of lane l's v (l the same on every lane)
+VH_DEV int at_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+// the largest / the sum over the four lanes of a head (lanes l, l + 16, l + 32, l + 48)
+VH_DEV float head_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+VH_DEV float head_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// What an output is multiplied by at the end: nothing attended, zeros; every
+// score -inf (no weight at all), a NaN, as the softmax of them is.
+VH_DEV float inverse(float M, float L) {
+    return M == -INFINITY ? 0.0f : L == 0.0f ? __builtin_nanf("") : 1.0f / L;
+}
+
+// x split into NP truncated 16-bit parts, the operand words of each; x >= 0
+// elements stay >= 0. Zero parts of a nonzero x become the least value.
+template <uint32_t T, int NP>
+VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        float a = x[j], b = x[j + 1];
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            if constexpr (T == VIREO_PAGED_BF16) {
+                if (p) {  // 2^-126, of the value's sign
+                    a = copysignf(fmaxf(fabsf(a), 1.17549435e-38f), x[j]);
+                    b = copysignf(fmaxf(fabsf(b), 1.17549435e-38f), x[j + 1]);
+                }
+                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+                w[p][j / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);  // the high halves
+                a -= __uint_as_float(ua & 0xffff0000u);
+                b -= __uint_as_float(ub & 0xffff0000u);
+            } else {
+                if (p) {  // 2^-24
+                    a = copysignf(fmaxf(fabsf(a), 5.9604645e-8f), x[j]);
+                    b = copysignf(fmaxf(fabsf(b), 5.9604645e-8f), x[j + 1]);
+                }
+                const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+                w[p][j / 2] = __builtin_bit_cast(uint32_t, h);
+                a -= float(h[0]);
+                b -= float(h[1]);
+            }
+        }
+    }
+}
+
+// D: head size; T: the cache's type; QF: fp32 queries and results (else T's)
+template <int D, uint32_t T, bool QF>
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
+    constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
+    constexpr int QP = QF ? 3 : 1;                       // parts of a query
+    constexpr int WP = QF && T == VIREO_PAGED_BF16 ? 3 : 2;  // parts of a weight
+    constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
+    __shared__ __align__(16) float red[2][16][RS];
+    __shared__ float2 wml[4][16];
+    if (a.head->tag != a.tag) return;  // not this plan's split
+    const int item = blockIdx.x;
+    const PlanItem it = a.items[item];
+    if (item >= a.head->n_items) return;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int g = blockIdx.y / a.tiles, z = blockIdx.y % a.tiles;
+    const int seq = it.seq & 0x7fffffff, h0 = g * a.hpg + z * 16, nh = min(16, a.hpg - z * 16);
+    const int shift = a.shift, G = 1 << shift;
+
+    // the queries: column col's head, dimensions 32 s + 8 grp .. + 7 of step s
+    u32x4 qw[QP][KS];
+    float c = a.c;
+    {
+        const int64_t qo = seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp;
+        if constexpr (QF) {
+            float x[KS][8], big = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                ld8(a.q, VIREO_PAGED_F32, qo + 32 * s, x[s]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[s][j]));
+            }
+            if constexpr (T == VIREO_PAGED_F16) {
+                // under a power of two that takes the head's largest into [2^14, 2^15)
+                big = head_max(big);
+                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+                const int e1 = e / 2;  // in two steps: 2^e alone may leave fp32's range
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
+                c = ldexpf(ldexpf(c, -e1), e1 - e);
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 w[QP];
+                split8<T, QP>(x[s], w);
+#pragma unroll
+                for (int p = 0; p < QP; p++) qw[p][s] = w[p];
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; s++) qw[0][s] = ldu4(static_cast<const uint16_t *>(a.q) + qo + 32 * s);
+        }
+    }
+
+    // the wave's tiles, and the blocks behind them, 64 at a time: lane e holds
+    // block e0 + e of the sequence (or of its list) and how many of its slots
+    // are attended (0: not a block)
+    const int T0 = (it.end - it.begin + 31) >> 5;
+    const int i0 = T0 * wv / 4, i1 = T0 * (wv + 1) / 4;
+    const int32_t *tab = a.table + size_t(it.row) * a.max_blocks;
+    const int length = a.lists ? a.len[it.row] : 0;
+    const int32_t *list = a.lists ? a.lists + (size_t(seq) * a.n_kv + g) * a.list_blocks : nullptr;
+    int e0 = 0, blk = 0, cnt = 0;
+    auto blocks_from = [&](int e) {
+        e0 = e;
+        const int mine = e + lane;
+        int b = -1, n = 0;
+        if (int64_t(mine) << shift < it.end) {
+            b = mine;
+            n = min(G, it.end - (mine << shift));
+            if (list) {
+                b = list[mine];
+                n = b >= 0 && b < a.max_blocks ? min(max(length - (b << shift), 0), G) : 0;
+            }
+        }
+        blk = n > 0 ? tab[b] : -1;
+        cnt = blk >= 0 && blk < a.n_blocks ? n : 0;
+        if (cnt == 0) blk = 0;
+    };
+    // tile i's two 16-token halves: the blocks they lie in, and where in them (a
+    // tile has at most two blocks of 16 slots)
+    const size_t head_tile = size_t(D) << shift;  // elements of a block of one kv head
+    struct Where {
+        size_t base[2];  // element of the half's block
+        int off[2];      // its first slot
+        int n[2];        // its slots that are attended, of 16
+    };
+    auto where = [&](int i) {
+        Where w;
+        const int t = it.begin + 32 * i;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int tu = t + 16 * u, e = (tu >> shift) - e0;
+            w.off[u] = tu & (G - 1);
+            w.base[u] = (size_t(at_lane(blk, e)) * a.n_kv + g) * head_tile;
+            w.n[u] = min(max(at_lane(cnt, e) - w.off[u], 0), 16);
+        }
+        return w;
+    };
+    // the lane's rows of K: row r = col of product u is token 8 (r / 4) + 4 u + r % 4 of the tile
+    const int kt = 8 * ((col >> 2) & 1) + (col & 3), khalf = col >> 3;
+    u32x4 kk[2][KS], vv[DT];
+    auto load_k = [&](const Where &w) {
+        const size_t base = khalf ? w.base[1] : w.base[0];
+        const int off = khalf ? w.off[1] : w.off[0];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint16_t *p = a.k + base + size_t(off + kt + 4 * u) * D + 8 * grp;
+#pragma unroll
+            for (int s = 0; s < KS; s++) kk[u][s] = ldu4(p + 32 * s);
+        }
+    };
+    auto load_v = [&](const Where &w) {
+        const size_t base = grp >> 1 ? w.base[1] : w.base[0];
+        const int off = (grp >> 1 ? w.off[1] : w.off[0]) + 8 * (grp & 1);
+        const uint16_t *p = a.v + base + (size_t(col) << shift) + off;
+#pragma unroll
+        for (int d = 0; d < DT; d++) vv[d] = ldu4(p + (size_t(16 * d) << shift));
+    };
+
+    float m = kLowest, l = 0.0f;
+    bool seen = false;  // a token was attended
+    f32x4 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (i0 < i1) {
+        blocks_from((it.begin + 32 * i0) >> shift);
+        Where w = where(i0);
+        load_k(w);
+        load_v(w);
+        for (int i = i0; i < i1; i++) {
+            f32x4 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = QP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int k = 0; k < KS; k++) s[u] = El<T>::mfma(kk[u][k], qw[p][k], s[u]);
+            }
+            const bool more = i + 1 < i1;
+            Where next = w;
+            if (more) {
+                if (((it.begin + 32 * i + 63) >> shift) - e0 >= 64) blocks_from((it.begin + 32 * (i + 1)) >> shift);
+                next = where(i + 1);
+                load_k(next);
+            }
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3];
+            const bool whole = w.n[0] == 16 && w.n[1] == 16;  // the same on every lane
+            // slots of the lane's 8 that are attended
+            const int nv = whole ? 8 : min(max((grp >> 1 ? w.n[1] : w.n[0]) - 8 * (grp & 1), 0), 8);
+            seen |= w.n[0] + w.n[1] > 0;
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = j < nv ? x[j] : -INFINITY;
+                // what lies in the other slots is not to meet a weight of 0: it may be an infinity or a NaN
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t keep = nv >= 2 * j + 2 ? 0xffffffffu : nv == 2 * j + 1 ? 0xffffu : 0u;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) vv[d][j] &= keep;
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) mx = fmaxf(mx, x[j]);
+            const float mn = fmaxf(m, head_max(mx) * c);
+            const float cr = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            // fp16's parts: weights up to 2^14, so that small ones keep their bits
+            const float up = T == VIREO_PAGED_F16 ? 14.0f - m : -m;
+            float ps = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, up));
+                ps += x[j];
+            }
+            l = fmaf(l, cr, ps);
+            u32x4 pw[WP];
+            split8<T, WP>(x, pw);
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] *= cr;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int p = WP - 1; p >= 0; p--) acc[d] = El<T>::mfma(vv[d], pw[p], acc[d]);
+            w = next;
+            if (more) load_v(w);
+        }
+    }
+    l = head_sum(l);
+    if (T == VIREO_PAGED_F16) l = l * 0x1p-14f;
+    // the waves' maxima; -inf marks a wave that attended nothing
+    if (grp == 0) wml[wv][col] = make_float2(seen ? m : -INFINITY, l);
+    __syncthreads();
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) M = fmaxf(M, wml[w][col].x);
+    float f = 0.0f;
+    if (M > -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float2 o = wml[w][col];
+            const float fw = __builtin_amdgcn_exp2f(o.x - M);
+            L = fmaf(o.y, fw, L);
+            f = w == wv ? fw : f;
+        }
+    }
+    if (T == VIREO_PAGED_F16) f *= 0x1p-14f;
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[d] *= f;
+    // sums of the four waves' outputs as (0 + 2) + (1 + 3)
+#pragma unroll
+    for (int half = 2; half >= 1; half--) {
+        if (wv >= half && wv < 2 * half) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(&red[wv - half][col][16 * d + 4 * grp]) = acc[d];
+        }
+        __syncthreads();
+        if (wv < half) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] += *reinterpret_cast<const f32x4 *>(&red[wv][col][16 * d + 4 * grp]);
+        }
+        __syncthreads();
+    }
+    if (wv != 0 || col >= nh) return;
+    const int h = h0 + col;
+    if (it.seq < 0) {  // the sequence's only item
+        const float inv = inverse(M, L);
+        const int64_t o = seq * a.out_stride + int64_t(h) * D + 4 * grp;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const f32x4 y = acc[d] * inv;
+            if constexpr (QF) {
+                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + o + 16 * d) = y;
+            } else {
+                u32x2 w;
+                w[0] = El<T>::pack(y[0], y[1]);
+                w[1] = El<T>::pack(y[2], y[3]);
+                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + o + 16 * d) = w;
+            }
+        }
+        return;
+    }
+    const size_t ph = size_t(item) * a.n_heads + h;
+    if (grp == 0) a.ml[ph] = make_float2(M, L);
+#pragma unroll
+    for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(a.part + ph * D + 16 * d + 4 * grp) = acc[d];
+}
+
+// A workgroup per (sequence, head) joins its items in order: thread groups of
+// D / 4 take every NG-th item, four dimensions a thread, and are added in order.
+template <int D, uint32_t T, bool QF>
+__global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
+    constexpr int ND = D / 4, NG = 256 / ND;
+    __shared__ f32x4 red[NG][ND];
+    __shared__ float rl[NG];
+    if (a.head->tag != a.tag) return;
+    const int seq = blockIdx.x / a.n_heads, h = blockIdx.x - seq * a.n_heads;
+    const int f0 = a.first[seq], n = a.first[seq + 1] - f0;
+    if (n == 1) return;
+    const int dq = threadIdx.x % ND, grp = threadIdx.x / ND;
+    float M = -INFINITY;
+    for (int i = 0; i < n; i++) M = fmaxf(M, a.ml[size_t(f0 + i) * a.n_heads + h].x);
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    float L = 0.0f;
+    if (M > -INFINITY)
+        for (int i = grp; i < n; i += NG) {
+            const size_t ph = size_t(f0 + i) * a.n_heads + h;
+            const float2 ml = a.ml[ph];
+            const float f = __builtin_amdgcn_exp2f(ml.x - M);
+            L = fmaf(ml.y, f, L);
+            y += *reinterpret_cast<const f32x4 *>(a.part + ph * D + 4 * dq) * f;
+        }
+    red[grp][dq] = y;
+    if (dq == 0) rl[grp] = L;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int u = 1; u < NG; u++) {
+        y += red[u][dq];
+        L += rl[u];
+    }
+    y *= inverse(M, L);
+    const int64_t o = seq * a.out_stride + int64_t(h) * D + 4 * dq;
+    if constexpr (QF) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + o) = y;
+    } else {
+        u32x2 w;
+        w[0] = El<T>::pack(y[0], y[1]);
+        w[1] = El<T>::pack(y[2], y[3]);
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + o) = w;
+    }
+}
+
+template <int D, uint32_t T, bool QF>
+void launch_attend(const AttendArgs &a, int cap, int n, hipStream_t s) {
+    hipLaunchKernelGGL((attend_kernel<D, T, QF>), dim3(cap, a.n_kv * a.tiles), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
+}
+
+template <int D>
+void launch_types(uint32_t cache, const AttendArgs &a, int cap, int n, hipStream_t s) {
+    const bool f = a.type == VIREO_PAGED_F32;
+    if (cache == VIREO_PAGED_BF16)
+        f ? launch_attend<D, VIREO_PAGED_BF16, true>(a, cap, n, s) : launch_attend<D, VIREO_PAGED_BF16, false>(a, cap, n, s);
+    else
+        f ? launch_attend<D, VIREO_PAGED_F16, true>(a, cap, n, s) : launch_attend<D, VIREO_PAGED_F16, false>(a, cap, n, s);
+}
+
+}  // namespace
+
+extern "C" int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_plan *p, const void *q, uint32_t type,
+                                  int64_t q_stride, float scale, const int32_t *lists, void *out, int64_t out_stride,
+                                  void *stream) {
+    if (!vh_cache_ok(c) || !vh_plan_ok(p) || !p->mem || (reinterpret_cast<uintptr_t>(p->mem) & 255u) ||
+        c->n_kv_heads != p->n_kv_heads || c->head_size != p->head_size || c->block_tokens != p->table->block_tokens ||
+        c->n_blocks != p->table->n_blocks || (type != VIREO_PAGED_F32 && type != c->type) ||
+        !vh_rows_ok(q, type, q_stride, p->n_heads, p->head_size, p->n) ||
+        !vh_rows_ok(out, type, out_stride, p->n_heads, p->head_size, p->n) || !(scale > 0.0f && scale < INFINITY) ||
+        (lists != nullptr) != (p->list_blocks > 0))
+        return -EINVAL;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const PlanView v = vh_plan_view(p);
+    int shift = 4;
+    while ((1 << shift) < c->block_tokens) shift++;
+    const AttendArgs a{static_cast<const uint16_t *>(c->k), static_cast<const uint16_t *>(c->v), c->n_blocks,
+                       c->n_kv_heads, shift, p->table->blocks, p->table->len, p->table->max_blocks, lists,
+                       p->list_blocks, q, q_stride, scale * kLog2e, p->n_heads, p->n_heads / p->n_kv_heads,
+                       vh_plan_head_tiles(p), out, out_stride, type, v.head, v.items, v.first, v.tag, v.part, v.ml};
+    if (c->head_size == 64) launch_types<64>(c->type, a, v.cap, p->n, s);
+    else if (c->head_size == 128) launch_types<128>(c->type, a, v.cap, p->n, s);
+    else launch_types<256>(c->type, a, v.cap, p->n, s);
+    return vh_finish(s, vh_check(hipGetLastError()));
+}
