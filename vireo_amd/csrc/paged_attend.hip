@@ -127,13 +127,16 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
     __shared__ __align__(16) float red[2][16][RS];
     __shared__ float2 wml[4][16];
-    if (a.head->tag != a.tag) return;  // not this plan's split
-    const int item = blockIdx.x;
+    // heads vary fastest: a block's kv heads are neighbours in memory, and the
+    // plan's unused items come last
+    const int item = blockIdx.y, hg = blockIdx.x;
+    const uint32_t tag = a.head->tag;
+    const int n_items = a.head->n_items;
     const PlanItem it = a.items[item];
-    if (item >= a.head->n_items) return;
+    if (tag != a.tag || item >= n_items) return;  // not this plan's split, or not an item of it
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int g = blockIdx.y / a.tiles, z = blockIdx.y % a.tiles;
+    const int g = hg / a.tiles, z = hg - g * a.tiles;
     const int seq = it.seq & 0x7fffffff, h0 = g * a.hpg + z * 16, nh = min(16, a.hpg - z * 16);
     const int shift = a.shift, G = 1 << shift;
 
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
 
 template <int D, uint32_t T, bool QF>
 void launch_attend(const AttendArgs &a, int cap, int n, hipStream_t s) {
-    hipLaunchKernelGGL((attend_kernel<D, T, QF>), dim3(cap, a.n_kv * a.tiles), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attend_kernel<D, T, QF>), dim3(a.n_kv * a.tiles, cap), dim3(256), 0, s, a);
     hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
 }
 

@@ -274,15 +274,21 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const i
 }
 
 // One workgroup: cut the batch into items. A sequence of u units (kPagedUnit
-// tokens) gets ceil(u / S) items, S the least that gives at most `slots` items
-// beside one per sequence; its units are dealt evenly. LDS: items' prefix sums
-// [n + 1], tokens [n], rows [n].
-__global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int slots,
-                                                        int list_blocks, PlanHead *__restrict__ head,
+// tokens) gets ceil(u / S) items and its units are dealt evenly over them. S is
+// the batch's units / `whole`, or up to an eighth more, if the items then number
+// at most `whole`: each CU has one, and they end together. Sequences that do not
+// divide so (short ones beside long ones) are cut finer, S = units / `fine`, so that
+// workgroups that end early take up others: 131 071 tokens alone 111 us (2 layers)
+// whole and 136 fine, 16 equal sequences 79 and 84; 64 sequences of 500 to 30 001
+// tokens 408 and 353, 23 of 1 to 8 191 67 and 59. Between the two, 131 071 tokens take 113 at
+// 512, 121 at 1 024 and 162 at 4 096 workgroups, the 64 sequences 396, 364 and 354.
+// LDS: items' prefix sums [n + 1], tokens [n], rows [n].
+__global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int whole,
+                                                        int fine, int list_blocks, PlanHead *__restrict__ head,
                                                         int32_t *__restrict__ first, PlanItem *__restrict__ items,
                                                         uint32_t tag) {
     extern __shared__ uint32_t lds[];
-    __shared__ uint32_t wsum[2][kThreads / 64];
+    __shared__ uint32_t wsum[2][kThreads / 64], many[3];
     uint32_t *fst = lds, *tok = fst + n + 1;
     int *rw = reinterpret_cast<int *>(tok + n);
     const int tid = threadIdx.x;
@@ -303,7 +309,28 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
         block_scan((tokens + kPagedUnit - 1) / kPagedUnit, wsum[(c / kThreads) & 1], &all);
         total = add_sat(total, all);
     }
-    const uint32_t S = max((total + slots - 1) / slots, 1u);
+    // the least S of three that gives at most `whole` items
+    if (tid < 3) many[tid] = 0;
+    __syncthreads();
+    uint32_t tries[3], mine[3] = {};
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        const uint64_t s16 = uint64_t(total) * (16 + k);
+        tries[k] = uint32_t(max((s16 + 16 * whole - 1) / (16 * whole), uint64_t(1)));
+    }
+    for (int i = tid; i < n; i += kThreads) {
+        const uint32_t u = (tok[i] + kPagedUnit - 1) / kPagedUnit;
+#pragma unroll
+        for (int k = 0; k < 3; k++) mine[k] += (u + tries[k] - 1) / tries[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+        if (mine[k]) atomicAdd(&many[k], mine[k]);
+    __syncthreads();
+    uint32_t S = max((total + fine - 1) / fine, 1u);
+#pragma unroll
+    for (int k = 2; k >= 0; k--)
+        if (many[k] <= uint32_t(whole)) S = tries[k];
     uint32_t sum = 0;
     for (int c = 0; c < n; c += kThreads) {
         const int i = c + tid;
@@ -354,13 +381,13 @@ int allow_lds(F *f, size_t bytes) {
                                         int(bytes)));
 }
 
-// Workgroups that a plan aims at over all kv heads: kPagedGroups (two per CU of
-// 256 with their registers, and as many again to even out their ends).
-constexpr int kPagedGroups = 1024;
-int plan_slots(const vireo_paged_plan *p) {
-    const int s = kPagedGroups / (p->n_kv_heads * vh_plan_head_tiles(p));
+// Items that a plan aims at per kv head (and tile of 16 query heads): whole, one
+// workgroup per CU over all of them; fine, eight.
+int plan_slots(const vireo_paged_plan *p, int groups) {
+    const int s = groups / (p->n_kv_heads * vh_plan_head_tiles(p));
     return s > 1 ? s : 1;
 }
+constexpr int kWholeGroups = 256, kFineGroups = 2048;
 
 }  // namespace
 
@@ -382,7 +409,10 @@ PlanView vh_plan_view(const vireo_paged_plan *p) {
         at += (bytes + 255) & ~int64_t(255);
         return q;
     };
-    v.cap = plan_slots(p) + p->n;
+    // no more items than units that the table (or the lists) can hold
+    const int64_t most = p->list_blocks && p->list_blocks < p->table->max_blocks ? p->list_blocks : p->table->max_blocks;
+    const int64_t units = (most * p->table->block_tokens + kPagedUnit - 1) / kPagedUnit * p->n;
+    v.cap = int(units < plan_slots(p, kFineGroups) + p->n ? units : plan_slots(p, kFineGroups) + p->n);
     v.head = reinterpret_cast<PlanHead *>(take(sizeof(PlanHead)));
     v.first = reinterpret_cast<int32_t *>(take(int64_t(p->n + 1) * 4));
     v.items = reinterpret_cast<PlanItem *>(take(int64_t(v.cap) * sizeof(PlanItem)));
@@ -450,7 +480,7 @@ extern "C" int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream) 
     hipStream_t s = static_cast<hipStream_t>(stream);
     const PlanView v = vh_plan_view(p);
     const size_t lds = 4 * size_t(p->n + 1) + 8 * size_t(p->n);
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n, plan_slots(p),
-                       p->list_blocks, v.head, v.first, v.items, v.tag);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n,
+                       plan_slots(p, kWholeGroups), plan_slots(p, kFineGroups), p->list_blocks, v.head, v.first, v.items, v.tag);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
