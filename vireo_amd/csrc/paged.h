@@ -101,6 +101,8 @@ struct El<VIREO_PAGED_F16> {
     }
 };
 VH_DEV u32x4 ldu4(const void *p) { return *reinterpret_cast<const u32x4 *>(p); }
+// with the non-temporal hint: what a launch reads once
+VH_DEV u32x4 ldu4_once(const void *p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)); }
 // 8 consecutive elements of a type known at run time (the same for the whole launch) as floats
 VH_DEV void ld8(const void *p, uint32_t type, int64_t i, float (&x)[8]) {
     if (type == VIREO_PAGED_F32) {
@@ -126,12 +128,13 @@ VH_DEV u32x4 pack8(const float (&x)[8], uint32_t type) {
                                         : El<VIREO_PAGED_F16>::pack(x[2 * j], x[2 * j + 1]);
     return w;
 }
-VH_DEV void st8(void *p, uint32_t type, int64_t i, const float (&x)[8]) {
+// 8 elements stored with the non-temporal hint
+VH_DEV void st8_once(void *p, uint32_t type, int64_t i, const float (&x)[8]) {
     if (type == VIREO_PAGED_F32) {
         f32x4 *d = reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i);
-        d[0] = f32x4{x[0], x[1], x[2], x[3]};
-        d[1] = f32x4{x[4], x[5], x[6], x[7]};
+        __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, d);
+        __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, d + 1);
     } else {
-        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + i) = pack8(x, type);
+        __builtin_nontemporal_store(pack8(x, type), reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + i));
     }
 }

@@ -9,13 +9,17 @@
 // takes hs / 16 lanes; a lane holds two runs of 8 values that are each other's
 // rotation partners (values 8 i .. and R/2 + 8 i ..), so loads and stores are
 // 16 bytes wide, the norm's sum is a few DPP adds and the rotation needs no
-// exchange. Bound by bytes for prompts and by its loads' round trip for a
-// decode batch.
+// exchange. Values go through LDS, 16 rows of a kv head at a time, so that a
+// store's lanes are neighbouring tokens of few dimensions. Queries are stored
+// with the non-temporal hint (4 093 rows, 84 MB: 22.9 -> 19.2 us, 4.4 TB/s with the
+// launch). Bound by bytes for prompts and by its loads' round trip for a decode batch.
 #include <hip/hip_runtime.h>
 #include <errno.h>
 #include "paged.h"
 
 namespace {
+
+constexpr int kVRows = 16;  // rows of a workgroup that stores values
 
 struct AppendArgs {
     vireo_paged_rows r;
@@ -23,107 +27,177 @@ struct AppendArgs {
     uint32_t cache_type;
     int n_kv, shift;  // block_tokens = 1 << shift
     int slots;        // of the pool
+    int qk_groups;    // workgroups of queries and keys; those behind store values
 };
 
+// A head of a row's queries or keys per group of lanes. (Four heads per group, the
+// rotation and norm weights read once for them: 4 093 rows 27.4 us, two 24.7, one 22.9:
+// the loads in flight count, not the ones that the L1 answers.)
 template <int HS>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+VH_DEV void append_qk(const AppendArgs &a) {
     constexpr int LPR = HS / 16;  // lanes per head row
     const vireo_paged_rows &r = a.r;
-    const int per_row = r.n_heads + 2 * a.n_kv, ln = threadIdx.x % LPR;
-    const int64_t total = int64_t(r.rows) * per_row;
-    int64_t idx = int64_t(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
-    const bool there = idx < total;
-    if (!there) idx = total - 1;  // every lane stays for the sums
-    const int t = int(idx / per_row), hh = int(idx - int64_t(t) * per_row);
-    const int kind = hh < r.n_heads ? 0 : hh < r.n_heads + a.n_kv ? 1 : 2;
-    const int h = kind == 0 ? hh : hh - r.n_heads - (kind == 2 ? a.n_kv : 0);
+    const int per_row = r.n_heads + a.n_kv, ln = threadIdx.x % LPR;
+    const uint32_t total = uint32_t(r.rows) * per_row, unit = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const bool there = unit < total;  // every lane stays for the sums
+    const uint32_t idx = there ? unit : total - 1;
+    const int t = int(idx / per_row), hh = int(idx - uint32_t(t) * per_row);
+    const bool key = hh >= r.n_heads;
+    const int h = key ? hh - r.n_heads : hh;
     const int slot = r.slots[t], pos = r.positions[t];
     // the lane's two runs of 8 values
     const int R = r.rotary, turned = R / 16;
     const int i0 = ln < turned ? 8 * ln : R + 16 * (ln - turned), i1 = ln < turned ? R / 2 + 8 * ln : i0 + 8;
-    float x[2][8];
-    const void *src = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
-    const int64_t at = t * (kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride) + int64_t(h) * HS;
-    ld8(src, r.type, at + i0, x[0]);
-    ld8(src, r.type, at + i1, x[1]);
-    const float *bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias;
-    const float *norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
-    if (bias) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[0][j] += bias[size_t(h) * HS + i0 + j], x[1][j] += bias[size_t(h) * HS + i1 + j];
+    float x[2][8], y[2][8];
+    {
+        const int64_t o = t * (key ? r.k_stride : r.q_stride) + int64_t(h) * HS;
+        ld8(key ? r.k : r.q, r.type, o + i0, x[0]);
+        ld8(key ? r.k : r.q, r.type, o + i1, x[1]);
     }
-    float ss = 0.0f;
+    if (const float *bias = key ? r.k_bias : r.q_bias) {
+        ld8(bias, VIREO_PAGED_F32, int64_t(h) * HS + i0, y[0]);
+        ld8(bias, VIREO_PAGED_F32, int64_t(h) * HS + i1, y[1]);
 #pragma unroll
-    for (int j = 0; j < 8; j++) ss = fmaf(x[0][j], x[0][j], fmaf(x[1][j], x[1][j], ss));
-    ss = group_sum<LPR>(ss);
-    if (norm) {
-        const float s = 1.0f / sqrtf(ss * (1.0f / HS) + r.eps);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[0][j] *= s * norm[i0 + j], x[1][j] *= s * norm[i1 + j];
+        for (int j = 0; j < 8; j++) x[0][j] += y[0][j], x[1][j] += y[1][j];
     }
-    if (kind < 2 && ln < turned && pos >= 0 && pos < r.max_pos) {
+    if (const float *norm = key ? r.k_norm : r.q_norm) {
+        ld8(norm, VIREO_PAGED_F32, i0, y[0]);
+        ld8(norm, VIREO_PAGED_F32, i1, y[1]);
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss = fmaf(x[0][j], x[0][j], fmaf(x[1][j], x[1][j], ss));
+        const float s = 1.0f / sqrtf(group_sum<LPR>(ss) * (1.0f / HS) + r.eps);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[0][j] *= s * y[0][j], x[1][j] *= s * y[1][j];
+    }
+    if (ln < turned && pos >= 0 && pos < r.max_pos) {
         const float *tab = r.rope + size_t(pos) * R + 8 * ln;
+        ld8(tab, VIREO_PAGED_F32, 0, y[0]);
+        ld8(tab, VIREO_PAGED_F32, R / 2, y[1]);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float c = tab[j], s = tab[R / 2 + j], lo = x[0][j], hi = x[1][j];
-            x[0][j] = lo * c - hi * s;
-            x[1][j] = lo * s + hi * c;
+            const float lo = x[0][j], hi = x[1][j];
+            x[0][j] = lo * y[0][j] - hi * y[1][j];
+            x[1][j] = lo * y[1][j] + hi * y[0][j];
         }
     }
     if (!there || slot < 0 || slot >= a.slots) return;
-    if (kind == 0) {
-        const int64_t o = t * r.q_out_stride + int64_t(h) * HS;
-        st8(r.q_out, r.q_out_type, o + i0, x[0]);
-        st8(r.q_out, r.q_out_type, o + i1, x[1]);
-        return;
-    }
-    const int G = 1 << a.shift, off = slot & (G - 1);
-    const size_t tile = (size_t(slot >> a.shift) * a.n_kv + h) * size_t(HS) * G;
-    const u32x4 w0 = pack8(x[0], a.cache_type), w1 = pack8(x[1], a.cache_type);
-    if (kind == 1) {
-        uint16_t *k = a.k + tile + size_t(off) * HS;
-        *reinterpret_cast<u32x4 *>(k + i0) = w0;
-        *reinterpret_cast<u32x4 *>(k + i1) = w1;
+    if (key) {
+        const int G = 1 << a.shift, off = slot & (G - 1);
+        uint16_t *k = a.k + ((size_t(slot >> a.shift) * a.n_kv + h) * G + off) * HS;
+        *reinterpret_cast<u32x4 *>(k + i0) = pack8(x[0], a.cache_type);
+        *reinterpret_cast<u32x4 *>(k + i1) = pack8(x[1], a.cache_type);
     } else {
-        uint16_t *v = a.v + tile + off;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            v[size_t(i0 + j) * G] = uint16_t(w0[j / 2] >> (16 * (j & 1)));
-            v[size_t(i1 + j) * G] = uint16_t(w1[j / 2] >> (16 * (j & 1)));
-        }
+        const int64_t o = t * r.q_out_stride + int64_t(h) * HS;
+        st8_once(r.q_out, r.q_out_type, o + i0, x[0]);
+        st8_once(r.q_out, r.q_out_type, o + i1, x[1]);
     }
 }
 
-// The mean key of each block whose last slot a row wrote, from its keys as
-// stored (so a block has the same mean however its tokens came): a thread per
-// 8 dimensions of a kv head adds the block's tokens in order in fp32.
-__global__ void __launch_bounds__(256) means_kernel(const int32_t *__restrict__ slots, int n_slots, int shift, int n_kv,
-                                                    int hs, uint32_t type, const uint16_t *__restrict__ k,
-                                                    uint16_t *__restrict__ means) {
-    const int slot = slots[blockIdx.x], G = 1 << shift;
-    if (slot < 0 || slot >= n_slots || (slot & (G - 1)) != G - 1) return;
-    const int per = hs / 8;
-    const size_t blk = size_t(slot >> shift);
-    for (int i = threadIdx.x; i < n_kv * per; i += 256) {
-        const uint16_t *src = k + (blk * n_kv + i / per) * size_t(hs) * G + (i % per) * 8;
-        float sum[8] = {};
-#pragma unroll 8
-        for (int g = 0; g < G; g++) {
-            float x[8];
-            ld8(src, type, int64_t(g) * hs, x);
+// kVRows rows of one kv head's values: read row by row, stored dimension by
+// dimension, 16 lanes a dimension's tokens (rows of one block lie side by side)
+template <int HS>
+VH_DEV void append_v(const AppendArgs &a) {
+    constexpr int RS = HS / 2 + 1;  // words of an LDS row: a column's 16 rows on different banks
+    __shared__ uint32_t tile[kVRows * RS];
+    const vireo_paged_rows &r = a.r;
+    const int unit = blockIdx.x - a.qk_groups, h = unit % a.n_kv, t0 = unit / a.n_kv * kVRows;
+    constexpr int CH = HS / 8;  // runs of 8 values of a row
+    for (int i = threadIdx.x; i < kVRows * CH; i += 256) {
+        const int t = t0 + i / CH, j0 = i % CH * 8;
+        if (t >= r.rows) break;
+        float x[8];
+        ld8(r.v, r.type, t * r.v_stride + int64_t(h) * HS + j0, x);
+        if (r.v_bias) {
+            float b[8];
+            ld8(r.v_bias, VIREO_PAGED_F32, int64_t(h) * HS + j0, b);
 #pragma unroll
-            for (int j = 0; j < 8; j++) sum[j] += x[j];
+            for (int j = 0; j < 8; j++) x[j] += b[j];
         }
+        const u32x4 w = pack8(x, a.cache_type);
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum[j] *= 1.0f / float(G);  // a power of two: exact
-        st8(means, type, int64_t(blk * n_kv * hs) + int64_t(i) * 8, sum);
+        for (int j = 0; j < 4; j++) tile[(i / CH) * RS + j0 / 2 + j] = w[j];
+    }
+    const int tt = threadIdx.x & 15, t = t0 + tt;
+    const int slot = t < r.rows ? r.slots[t] : -1;
+    __syncthreads();
+    if (slot < 0 || slot >= a.slots) return;
+    const int G = 1 << a.shift;
+    uint16_t *v = a.v + (size_t(slot >> a.shift) * a.n_kv + h) * size_t(HS) * G + (slot & (G - 1));
+#pragma unroll 4
+    for (int j = 2 * (threadIdx.x >> 4); j < HS; j += 32) {
+        const uint32_t w = tile[tt * RS + j / 2];
+        v[size_t(j) * G] = uint16_t(w);
+        v[size_t(j + 1) * G] = uint16_t(w >> 16);
     }
 }
 
 template <int HS>
-void launch_append(const AppendArgs &a, hipStream_t s) {
-    const int64_t rows = int64_t(a.r.rows) * (a.r.n_heads + 2 * a.n_kv), per = 256 / (HS / 16);
-    hipLaunchKernelGGL(append_kernel<HS>, dim3(unsigned((rows + per - 1) / per)), dim3(256), 0, s, a);
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+    if (int(blockIdx.x) < a.qk_groups) append_qk<HS>(a);
+    else append_v<HS>(a);
+}
+
+// The mean key of each block whose last slot a row wrote, from its keys as
+// stored (so a block has the same mean however its tokens came). A workgroup
+// looks at kMeanRows rows for one kv head, a wave per row: 16 lanes a token's HS
+// values, four tokens at a time, added in order and then across the four.
+constexpr int kMeanRows = 16;
+template <int HS>
+__global__ void __launch_bounds__(256) means_kernel(const int32_t *__restrict__ slots, int rows, int n_slots, int shift,
+                                                    int n_kv, uint32_t type, const uint16_t *__restrict__ k,
+                                                    uint16_t *__restrict__ means) {
+    constexpr int E = HS / 16;  // values of a lane: E / 4 runs of 4, 64 apart
+    const int lane = threadIdx.x & 63, sub = lane & 15, tok = lane >> 4, h = blockIdx.y, G = 1 << shift;
+    for (int t = blockIdx.x * kMeanRows + (threadIdx.x >> 6); t < min(rows, int(blockIdx.x + 1) * kMeanRows); t += 4) {
+        const int slot = slots[t];
+        if (slot < 0 || slot >= n_slots || (slot & (G - 1)) != G - 1) continue;
+        const size_t head = size_t(slot >> shift) * n_kv + h;
+        const uint16_t *src = k + (head * G + tok) * HS + 4 * sub;
+        float sum[E] = {};
+#pragma unroll 4
+        for (int g = 0; g < G; g += 4)
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(src + size_t(g) * HS + 16 * e);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float2 f = type == VIREO_PAGED_BF16 ? El<VIREO_PAGED_BF16>::unpack(w[j])
+                                                              : El<VIREO_PAGED_F16>::unpack(w[j]);
+                    sum[e + 2 * j] += f.x;
+                    sum[e + 2 * j + 1] += f.y;
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            sum[e] += __shfl_xor(sum[e], 16);
+            sum[e] += __shfl_xor(sum[e], 32);
+            sum[e] *= 1.0f / float(G);  // a power of two: exact
+        }
+        if (tok == 0)
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                u32x2 w;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    w[j] = type == VIREO_PAGED_BF16 ? El<VIREO_PAGED_BF16>::pack(sum[e + 2 * j], sum[e + 2 * j + 1])
+                                                    : El<VIREO_PAGED_F16>::pack(sum[e + 2 * j], sum[e + 2 * j + 1]);
+                *reinterpret_cast<u32x2 *>(means + head * HS + 16 * e + 4 * sub) = w;
+            }
+    }
+}
+
+template <int HS>
+void launch_append(AppendArgs a, uint16_t *means, hipStream_t s) {
+    const vireo_paged_rows &r = a.r;
+    constexpr int kGroups = 256 / (HS / 16);  // head rows of a workgroup
+    const int64_t heads = int64_t(r.rows) * (r.n_heads + a.n_kv);
+    const int64_t values = int64_t((r.rows + kVRows - 1) / kVRows) * a.n_kv;
+    a.qk_groups = int((heads + kGroups - 1) / kGroups);
+    hipLaunchKernelGGL(append_kernel<HS>, dim3(unsigned(a.qk_groups + values)), dim3(256), 0, s, a);
+    if (means)
+        hipLaunchKernelGGL(means_kernel<HS>, dim3((r.rows + kMeanRows - 1) / kMeanRows, a.n_kv), dim3(256), 0, s,
+                           r.slots, r.rows, a.slots, a.shift, a.n_kv, a.cache_type, a.k, means);
 }
 
 }  // namespace
@@ -145,13 +219,11 @@ extern "C" int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_
     if (r->rows == 0) return vh_finish(s, 0);
     int shift = 4;
     while ((1 << shift) < c->block_tokens) shift++;
-    AppendArgs a{*r, static_cast<uint16_t *>(c->k), static_cast<uint16_t *>(c->v), c->type, c->n_kv_heads, shift,
-                 c->n_blocks * c->block_tokens};
-    if (hs == 64) launch_append<64>(a, s);
-    else if (hs == 128) launch_append<128>(a, s);
-    else launch_append<256>(a, s);
-    if (c->means)
-        hipLaunchKernelGGL(means_kernel, dim3(r->rows), dim3(256), 0, s, r->slots, a.slots, shift, c->n_kv_heads, hs,
-                           c->type, a.k, static_cast<uint16_t *>(c->means));
+    const AppendArgs a{*r, static_cast<uint16_t *>(c->k), static_cast<uint16_t *>(c->v), c->type, c->n_kv_heads, shift,
+                 c->n_blocks * c->block_tokens, 0};
+    uint16_t *means = static_cast<uint16_t *>(c->means);
+    if (hs == 64) launch_append<64>(a, means, s);
+    else if (hs == 128) launch_append<128>(a, means, s);
+    else launch_append<256>(a, means, s);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
