@@ -52,8 +52,12 @@ struct PlanItem {
     int32_t begin, end;  // tokens (of the listed blocks, where the plan has lists)
     int32_t seq;         // in the batch; bit 31: the sequence's only item
 };
+struct PlanSeq {
+    int32_t row, blocks;  // of the table; 0 blocks: an empty sequence, or not one
+};
 struct PlanView {
     PlanHead *head;
+    PlanSeq *seqs;    // [n]
     int32_t *first;   // [n + 1]
     PlanItem *items;  // [cap]
     uint32_t *keys;   // [n x n_kv_heads x max_blocks] ordered scores (plans with lists)
@@ -136,5 +140,86 @@ VH_DEV void st8_once(void *p, uint32_t type, int64_t i, const float (&x)[8]) {
         __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, d + 1);
     } else {
         __builtin_nontemporal_store(pack8(x, type), reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + i));
+    }
+}
+// the largest / the sum over the four lanes of a column (lanes l, l + 16, l + 32, l + 48)
+VH_DEV float head_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+VH_DEV float head_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// x split into NP truncated 16-bit parts, the operand words of each; x >= 0
+// elements stay >= 0. Zero parts of a nonzero x become the least value.
+template <uint32_t T, int NP>
+VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        float a = x[j], b = x[j + 1];
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            if constexpr (T == VIREO_PAGED_BF16) {
+                if (p) {  // 2^-126, of the value's sign
+                    a = copysignf(fmaxf(fabsf(a), 1.17549435e-38f), x[j]);
+                    b = copysignf(fmaxf(fabsf(b), 1.17549435e-38f), x[j + 1]);
+                }
+                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+                w[p][j / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);  // the high halves
+                a -= __uint_as_float(ua & 0xffff0000u);
+                b -= __uint_as_float(ub & 0xffff0000u);
+            } else {
+                if (p) {  // 2^-24
+                    a = copysignf(fmaxf(fabsf(a), 5.9604645e-8f), x[j]);
+                    b = copysignf(fmaxf(fabsf(b), 5.9604645e-8f), x[j + 1]);
+                }
+                const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+                w[p][j / 2] = __builtin_bit_cast(uint32_t, h);
+                a -= float(h[0]);
+                b -= float(h[1]);
+            }
+        }
+    }
+}
+
+// A matrix operand of queries of type F32 (QF) or T as parts of T: lane (col,
+// grp) loads values 32 s + 0 .. 7 from element `at` on (its head's, 8 grp in) for
+// each step s. fp32 queries over fp16 are taken under a power of two that brings the
+// head's largest into [2^14, 2^15); returns its exponent.
+constexpr int query_parts(bool f32) { return f32 ? 3 : 1; }
+template <int D, uint32_t T, bool QF>
+VH_DEV int load_queries(const void *q, int64_t at, u32x4 (&w)[query_parts(QF)][D / 32]) {
+    constexpr int KS = D / 32;
+    if constexpr (!QF) {
+#pragma unroll
+        for (int s = 0; s < KS; s++) w[0][s] = ldu4(static_cast<const uint16_t *>(q) + at + 32 * s);
+        return 0;
+    } else {
+        float x[KS][8], big = 0.0f;
+        int e = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            ld8(q, VIREO_PAGED_F32, at + 32 * s, x[s]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[s][j]));
+        }
+        if constexpr (T == VIREO_PAGED_F16) {
+            big = head_max(big);
+            if (big > 0.0f && big < INFINITY) e = 14 - ilogbf(big);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            u32x4 p[3];
+            split8<T, 3>(x[s], p);
+#pragma unroll
+            for (int k = 0; k < 3; k++) w[k][s] = p[k];
+        }
+        return e;
     }
 }

@@ -71,59 +71,17 @@ struct AttendArgs {
 
 // the wave's value of lane l's v (l the same on every lane)
 VH_DEV int at_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
-// the largest / the sum over the four lanes of a head (lanes l, l + 16, l + 32, l + 48)
-VH_DEV float head_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
-VH_DEV float head_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
-
 // What an output is multiplied by at the end: nothing attended, zeros; every
 // score -inf (no weight at all), a NaN, as the softmax of them is.
 VH_DEV float inverse(float M, float L) {
     return M == -INFINITY ? 0.0f : L == 0.0f ? __builtin_nanf("") : 1.0f / L;
 }
 
-// x split into NP truncated 16-bit parts, the operand words of each; x >= 0
-// elements stay >= 0. Zero parts of a nonzero x become the least value.
-template <uint32_t T, int NP>
-VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        float a = x[j], b = x[j + 1];
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-            if constexpr (T == VIREO_PAGED_BF16) {
-                if (p) {  // 2^-126, of the value's sign
-                    a = copysignf(fmaxf(fabsf(a), 1.17549435e-38f), x[j]);
-                    b = copysignf(fmaxf(fabsf(b), 1.17549435e-38f), x[j + 1]);
-                }
-                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-                w[p][j / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);  // the high halves
-                a -= __uint_as_float(ua & 0xffff0000u);
-                b -= __uint_as_float(ub & 0xffff0000u);
-            } else {
-                if (p) {  // 2^-24
-                    a = copysignf(fmaxf(fabsf(a), 5.9604645e-8f), x[j]);
-                    b = copysignf(fmaxf(fabsf(b), 5.9604645e-8f), x[j + 1]);
-                }
-                const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-                w[p][j / 2] = __builtin_bit_cast(uint32_t, h);
-                a -= float(h[0]);
-                b -= float(h[1]);
-            }
-        }
-    }
-}
-
 // D: head size; T: the cache's type; QF: fp32 queries and results (else T's)
 template <int D, uint32_t T, bool QF>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
     constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
-    constexpr int QP = QF ? 3 : 1;                       // parts of a query
+    constexpr int QP = query_parts(QF);
     constexpr int WP = QF && T == VIREO_PAGED_BF16 ? 3 : 2;  // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
     __shared__ __align__(16) float red[2][16][RS];
@@ -143,40 +101,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
 
     // the queries: column col's head, dimensions 32 s + 8 grp .. + 7 of step s
     u32x4 qw[QP][KS];
-    float c = a.c;
-    {
-        const int64_t qo = seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp;
-        if constexpr (QF) {
-            float x[KS][8], big = 0.0f;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                ld8(a.q, VIREO_PAGED_F32, qo + 32 * s, x[s]);
-#pragma unroll
-                for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[s][j]));
-            }
-            if constexpr (T == VIREO_PAGED_F16) {
-                // under a power of two that takes the head's largest into [2^14, 2^15)
-                big = head_max(big);
-                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
-                const int e1 = e / 2;  // in two steps: 2^e alone may leave fp32's range
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
-                c = ldexpf(ldexpf(c, -e1), e1 - e);
-            }
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                u32x4 w[QP];
-                split8<T, QP>(x[s], w);
-#pragma unroll
-                for (int p = 0; p < QP; p++) qw[p][s] = w[p];
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < KS; s++) qw[0][s] = ldu4(static_cast<const uint16_t *>(a.q) + qo + 32 * s);
-        }
-    }
+    const int e = load_queries<D, T, QF>(a.q, seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp, qw);
+    const float c = ldexpf(ldexpf(a.c, -(e / 2)), e / 2 - e);  // in two steps: 2^e alone may leave fp32's range
 
     // the wave's tiles, and the blocks behind them, 64 at a time: lane e holds
     // block e0 + e of the sequence (or of its list) and how many of its slots

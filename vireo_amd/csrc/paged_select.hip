@@ -11,12 +11,16 @@
 //
 // score_kernel: 16 lanes per mean key (16-bit, D / 16 consecutive values a
 // lane), four keys per group of 16 lanes; per query head the lanes' four sums are
-// transposed while they are reduced (5 exchanges instead of 16). Bound by the
-// read of the mean keys where the batch is large and by fp64 operations where
-// a kv head has many query heads.
-// choose_kernel: a workgroup per (sequence, kv head) finds the budget's lowest
-// key by four 8-bit digits from the top and writes the blocks in order. Bound
-// by its passes over the keys (L2) and their barriers.
+// transposed while they are reduced (5 exchanges instead of 16). 228 000 mean keys of
+// 128 (58 MB, 16 sequences of 9 000 to 65 536 tokens) against 4 heads each take 19.6 us
+// (24.2 with a block's kv heads far apart in the grid); against one head each 14.2,
+// which is the read; the rest is fp64. The fp64 matrix cores took 46.8 (140 cycles a 16x16x4 product),
+// and 16-bit matrix products that leave only the heads near the highest to fp64 33.9
+// (their operand reads 64 bytes of a key at a time).
+// choose_kernel: a workgroup per (sequence, kv head), its keys in registers,
+// finds the budget's lowest key by 8-bit digits of its distance from the lowest one
+// (two or three, where keys differ by their last bits four) and writes the blocks in
+// order by one prefix sum. Bound by its chain of loads, barriers and LDS atomics.
 #include <hip/hip_runtime.h>
 #include <errno.h>
 #include "paged.h"
@@ -30,9 +34,12 @@ constexpr int kThreads = 1024;  // of choose_kernel
 struct SelectArgs {
     const uint16_t *means;
     uint32_t cache_type;
-    int n_blocks, n_kv, shift;
-    const int32_t *ids, *table, *len;
-    int max_seqs, max_blocks;
+    int n_blocks, n_kv;
+    const int32_t *table;
+    int max_blocks;
+    const PlanHead *head;
+    const PlanSeq *seqs;
+    uint32_t tag;
     const void *q;
     uint32_t q_type;
     int64_t q_stride;
@@ -41,15 +48,6 @@ struct SelectArgs {
     uint32_t *keys;
     int32_t *lists;
 };
-
-// the sequence's blocks
-VH_DEV int blocks_have(const SelectArgs &a, int i, int *row) {
-    const int id = a.ids ? a.ids[i] : i;
-    if (id < 0 || id >= a.max_seqs) return 0;
-    *row = id;
-    const uint32_t len = uint32_t(max(a.len[id], 0));
-    return min(int((len + (1u << a.shift) - 1) >> a.shift), a.max_blocks);
-}
 
 // a float as an unsigned integer in the floats' order (-0 as 0)
 VH_DEV uint32_t ordered(float f) {
@@ -68,11 +66,10 @@ template <int D, uint32_t T>
 __global__ void __launch_bounds__(256) score_kernel(SelectArgs a) {
     constexpr int E = D / 16;
     __shared__ __align__(16) float qs[kHeads][D];
-    const int i = blockIdx.z, g = blockIdx.y;
-    int row = 0;
-    const int have = blocks_have(a, i, &row);
-    const int b0 = a.sinks + blockIdx.x * kScoreRows, hi = have - a.window;
-    if (have <= a.width || b0 >= hi) return;
+    const int i = blockIdx.z, g = blockIdx.x;  // a block's kv heads lie side by side
+    const PlanSeq sq = a.seqs[i];
+    const int row = sq.row, have = sq.blocks, b0 = a.sinks + blockIdx.y * kScoreRows, hi = have - a.window;
+    if (a.head->tag != a.tag || have <= a.width || b0 >= hi) return;
     const int lane = threadIdx.x & 63, sub = lane & 15;
     // the group's four mean keys: blocks b .. b + 3 (past the end: the last one again)
     const int b = b0 + 4 * int(threadIdx.x >> 4);
@@ -129,12 +126,17 @@ __global__ void __launch_bounds__(256) score_kernel(SelectArgs a) {
     if (sub < 4 && b + sub < hi) a.keys[(size_t(i) * a.n_kv + g) * a.max_blocks + b + sub] = ordered(float(best));
 }
 
+// Keys that a thread of choose_kernel holds in registers; a sequence with more
+// candidates reads them again in every pass.
+constexpr int kHeld = 8;
+
 __global__ void __launch_bounds__(kThreads) choose_kernel(SelectArgs a) {
-    __shared__ uint32_t hist[256], wsum[kThreads / 64];
-    __shared__ uint32_t found, left;
+    __shared__ uint32_t hist[2][256], wlo[kThreads / 64], whi[kThreads / 64];
+    __shared__ uint64_t wsum[kThreads / 64];
+    __shared__ uint32_t found, left, there;
     const int g = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    int row = 0;
-    const int have = blocks_have(a, i, &row);
+    const int have = a.seqs[i].blocks;
+    if (a.head->tag != a.tag) return;
     int32_t *list = a.lists + (size_t(i) * a.n_kv + g) * a.width;
     if (have <= a.width) {
         for (int x = tid; x < a.width; x += kThreads) list[x] = x < have ? x : -1;
@@ -142,23 +144,50 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(SelectArgs a) {
     }
     const int budget = a.width - a.sinks - a.window, n = have - a.sinks - a.window;  // n > budget
     const uint32_t *keys = a.keys + (size_t(i) * a.n_kv + g) * a.max_blocks + a.sinks;
+    // thread tid's candidates: x0 .. x0 + per - 1 (below n), in order
+    const int per = (n + kThreads - 1) / kThreads, x0 = tid * per, cnt = max(min(per, n - x0), 0);
+    const bool held = per <= kHeld;
+    uint32_t k[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) k[j] = held && j < cnt ? keys[x0 + j] : 0;
     for (int x = tid; x < a.sinks; x += kThreads) list[x] = x;
     for (int x = tid; x < a.window; x += kThreads) list[a.sinks + budget + x] = have - a.window + x;
     if (budget == 0) return;
-    // the budget-th highest key, digit by digit; `need` of the keys that share its digits so far are taken
-    uint32_t key = 0, need = uint32_t(budget);
-    for (int d = 24; d >= 0; d -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int x = tid; x < n; x += kThreads) {
-            const uint32_t k = keys[x];
-            if (d == 24 || (k >> (d + 8)) == (key >> (d + 8))) atomicAdd(&hist[(k >> d) & 255], 1u);
+    auto each = [&](auto f) {
+        if (held) {
+#pragma unroll
+            for (int j = 0; j < kHeld; j++)
+                if (j < cnt) f(x0 + j, k[j]);
+        } else {
+            for (int j = 0; j < cnt; j++) f(x0 + j, keys[x0 + j]);
         }
+    };
+    // the range of the keys: digits are of key - lowest, so that they spread
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each([&](int, uint32_t key) { lo = min(lo, key), hi = max(hi, key); });
+    hi = wave_max_u(hi);
+    lo = ~wave_max_u(~lo);
+    if (lane == 0) wlo[wv] = lo, whi[wv] = hi;
+    if (tid < 512) hist[tid >> 8][tid & 255] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) lo = min(lo, wlo[w]), hi = max(hi, whi[w]);
+    // `need` of the keys whose (key - lo) >> shift is `top` are taken, and all above
+    int shift = 32 - __clz(hi - lo);  // __clz(0) is 32
+    uint32_t top = 0, need = uint32_t(budget);
+    for (int pass = 0; shift > 0; pass++) {
+        const int bits = min(shift, 8);
+        uint32_t *now = hist[pass & 1];
+        shift -= bits;
+        each([&](int, uint32_t key) {
+            const uint32_t v = (key - lo) >> shift;
+            if (uint64_t(v) >> bits == top) atomicAdd(&now[v & ((1u << bits) - 1)], 1u);
+        });
         __syncthreads();
         if (wv == 0) {  // lane l: digits 255 - 4 l .. 252 - 4 l
             uint32_t c[4], sum = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum += c[j] = hist[255 - 4 * lane - j];
+            for (int j = 0; j < 4; j++) sum += c[j] = now[255 - 4 * lane - j];
             uint32_t upto = sum;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -168,42 +197,44 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(SelectArgs a) {
             uint32_t before = upto - sum;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (before < need && before + c[j] >= need) found = uint32_t(255 - 4 * lane - j), left = need - before;
+                if (before < need && before + c[j] >= need)
+                    found = uint32_t(255 - 4 * lane - j), left = need - before, there = c[j];
                 before += c[j];
             }
+        } else if (wv >= 4 && wv < 8) {
+            hist[(pass & 1) ^ 1][tid & 255] = 0;  // read last in the pass before
         }
         __syncthreads();
-        key |= found << d;
+        top = (top << bits) | found;
         need = left;
+        if (there == need) break;  // all of them: the lower digits do not matter
     }
-    // the keys above it and the first `need` equal ones, in order
+    // the keys above and the first `need` equal ones, in order: one prefix sum of both counts
     uint32_t above = 0, equal = 0;
-    for (int x0 = 0; x0 < n; x0 += kThreads) {
-        const int x = x0 + tid;
-        const uint32_t k = x < n ? keys[x] : 0;
-        const bool gt = x < n && k > key, eq = x < n && k == key;
-        // both counts in one word: at most 1024 each
-        const uint32_t mine = (gt ? 1u : 0u) | (eq ? 65536u : 0u);
-        uint32_t s = mine;
+    each([&](int, uint32_t key) {
+        const uint32_t v = uint32_t(uint64_t(key - lo) >> shift);
+        above += v > top, equal += v == top;
+    });
+    const uint64_t mine = (uint64_t(equal) << 32) | above;
+    uint64_t s = mine;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t u = __shfl_up(s, o);
-            if (lane >= o) s += u;
-        }
-        __syncthreads();  // wsum is free
-        if (lane == 63) wsum[wv] = s;
-        __syncthreads();
-        uint32_t before = s - mine, all = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / 64; w++) {
-            if (w < wv) before += wsum[w];
-            all += wsum[w];
-        }
-        const uint32_t eb = equal + (before >> 16), gb = above + (before & 65535u);
-        if (gt || (eq && eb < need)) list[a.sinks + gb + min(eb, need)] = a.sinks + x;
-        above += all & 65535u;
-        equal += all >> 16;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t u = __shfl_up(s, o);
+        if (lane >= o) s += u;
     }
+    if (lane == 63) wsum[wv] = s;
+    __syncthreads();
+    uint64_t before = s - mine;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++)
+        if (w < wv) before += wsum[w];
+    uint32_t gt = uint32_t(before), eq = uint32_t(before >> 32);
+    each([&](int x, uint32_t key) {
+        const uint32_t v = uint32_t(uint64_t(key - lo) >> shift);
+        const bool take = v > top || (v == top && eq < need);
+        if (take) list[a.sinks + gt + min(eq, need)] = a.sinks + x;
+        gt += v > top, eq += v == top;
+    });
 }
 
 }  // namespace
@@ -217,14 +248,13 @@ extern "C" int vireo_paged_select(const vireo_paged_cache *c, const vireo_paged_
         p->list_blocks == 0 || int64_t(sinks) + window > p->list_blocks || !lists)
         return -EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    int shift = 4;
-    while ((1 << shift) < c->block_tokens) shift++;
-    const SelectArgs a{static_cast<const uint16_t *>(c->means), c->type, c->n_blocks, c->n_kv_heads, shift, p->ids,
-                       p->table->blocks, p->table->len, p->table->max_seqs, p->table->max_blocks, q, type, q_stride,
-                       p->n_heads / p->n_kv_heads, sinks, window, p->list_blocks, vh_plan_view(p).keys, lists};
+    const PlanView v = vh_plan_view(p);
+    const SelectArgs a{static_cast<const uint16_t *>(c->means), c->type, c->n_blocks, c->n_kv_heads, p->table->blocks,
+                       p->table->max_blocks, v.head, v.seqs, v.tag, q, type, q_stride, p->n_heads / p->n_kv_heads, sinks,
+                       window, p->list_blocks, v.keys, lists};
     const int cand = p->table->max_blocks - sinks - window;
     if (p->table->max_blocks > p->list_blocks && p->list_blocks > sinks + window) {
-        const dim3 grid((cand + kScoreRows - 1) / kScoreRows, c->n_kv_heads, p->n);
+        const dim3 grid(c->n_kv_heads, (cand + kScoreRows - 1) / kScoreRows, p->n);
         const bool bf = c->type == VIREO_PAGED_BF16;
 #define SCORE(D)                                                                                                   \
     if (c->head_size == D) {                                                                                       \

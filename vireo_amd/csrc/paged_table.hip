@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const i
 // LDS: items' prefix sums [n + 1], tokens [n], rows [n].
 __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int whole,
                                                         int fine, int list_blocks, PlanHead *__restrict__ head,
+                                                        PlanSeq *__restrict__ seqs,
                                                         int32_t *__restrict__ first, PlanItem *__restrict__ items,
                                                         uint32_t tag) {
     extern __shared__ uint32_t lds[];
@@ -301,9 +302,11 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
             const int id = ids ? ids[i] : i;
             const bool ok = id >= 0 && id < t.max_seqs;
             if (ok) tokens = min(uint32_t(max(t.len[id], 0)), most);
-            if (list_blocks) tokens = uint32_t(min(blocks_of(tokens, t.shift), list_blocks)) << t.shift;
+            const int blocks = blocks_of(tokens, t.shift);
+            if (list_blocks) tokens = uint32_t(min(blocks, list_blocks)) << t.shift;
             tok[i] = tokens;
             rw[i] = ok ? id : 0;
+            seqs[i] = PlanSeq{rw[i], blocks};
         }
         uint32_t all;
         block_scan((tokens + kPagedUnit - 1) / kPagedUnit, wsum[(c / kThreads) & 1], &all);
@@ -414,6 +417,7 @@ PlanView vh_plan_view(const vireo_paged_plan *p) {
     const int64_t units = (most * p->table->block_tokens + kPagedUnit - 1) / kPagedUnit * p->n;
     v.cap = int(units < plan_slots(p, kFineGroups) + p->n ? units : plan_slots(p, kFineGroups) + p->n);
     v.head = reinterpret_cast<PlanHead *>(take(sizeof(PlanHead)));
+    v.seqs = reinterpret_cast<PlanSeq *>(take(int64_t(p->n) * sizeof(PlanSeq)));
     v.first = reinterpret_cast<int32_t *>(take(int64_t(p->n + 1) * 4));
     v.items = reinterpret_cast<PlanItem *>(take(int64_t(v.cap) * sizeof(PlanItem)));
     v.keys = reinterpret_cast<uint32_t *>(
@@ -481,6 +485,6 @@ extern "C" int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream) 
     const PlanView v = vh_plan_view(p);
     const size_t lds = 4 * size_t(p->n + 1) + 8 * size_t(p->n);
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n,
-                       plan_slots(p, kWholeGroups), plan_slots(p, kFineGroups), p->list_blocks, v.head, v.first, v.items, v.tag);
+                       plan_slots(p, kWholeGroups), plan_slots(p, kFineGroups), p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
