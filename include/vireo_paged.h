@@ -184,7 +184,8 @@ int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_plan *p, co
  * highest: the largest, over the kv head's query heads, of q . mean key, summed
  * in fp64 and rounded to fp32 (a NaN counts as -inf); of equal ones the lower
  * block first. A sequence of at most list_blocks blocks gets all of them, then
- * -1. c->means is required. Lengths are those at the plan's update. q as in
+ * -1. c->means is required. -E2BIG for a table of more than 65536 blocks a sequence
+ * beside sinks and window. Lengths are those at the plan's update. q as in
  * vireo_paged_attend. */
 int vireo_paged_select(const vireo_paged_cache *c, const vireo_paged_plan *p, const void *q, uint32_t type,
                        int64_t q_stride, int sinks, int window, int32_t *lists, void *stream);

@@ -463,7 +463,8 @@ def choose64(q, means, have, sinks, window, width):
 # (head size, heads, kv heads, block tokens, cache, query, sinks, window, budget, lengths)
 SELECT = [(128, 32, 4, 16, BF, BF, 1, 4, 32, [30001, 700, 590, 593, 0, 1]), (64, 8, 2, 16, HF, F32, 0, 1, 5, [3000, 97, 96, 111]),
           (256, 8, 1, 64, BF, F32, 2, 2, 16, [20011, 1281, 1280]), (128, 20, 1, 32, HF, HF, 0, 3, 0, [5000, 64]),
-          (64, 34, 2, 128, BF, BF, 3, 1, 9, [20000, 300]), (128, 4, 4, 16, BF, F32, 1, 2, 300, [70000, 5000])]
+          (64, 34, 2, 128, BF, BF, 3, 1, 9, [20000, 300]), (128, 4, 4, 16, BF, F32, 1, 2, 300, [70000, 5000]),
+          (64, 2, 1, 16, BF, BF, 1, 1, 40, [150000, 8200 * 16])]
 
 
 @pytest.mark.parametrize("d,H,KV,G,cache,query,sinks,window,budget,lens", SELECT)
@@ -518,6 +519,27 @@ def test_select_with_nan_and_equal_scores(cuda):
     b.q[:] = math.nan
     c.select(b.q, plan, lists, sinks=1, window=1)
     assert lists[0, 0].tolist() == list(range(11)) + [39]
+
+
+@pytest.mark.parametrize("blocks,levels,big", [(300, 1, 1.0), (300, 3, 1.0), (1500, 2, 1e30), (5000, 7, 1.0), (300, 2, math.inf)])
+def test_select_many_equal_scores(cuda, blocks, levels, big):
+    """Scores of few different values, infinite ones among them: the lower blocks of the last value that fits."""
+    b = Batch(cuda, [16 * blocks - 3], 2, 1, 64, 16, BF, F32, seed=blocks)
+    pages = torch.tensor(b.rows[b.ids[0]][:blocks], device=cuda)
+    means = torch.zeros((b.cache.n_blocks, 1, 64), dtype=BF, device=cuda)
+    value = torch.randint(levels, (blocks,), generator=gen(cuda, 1), device=cuda).float() - 1
+    means[pages, 0, 7] = torch.where(value == 0, 0.0, value * big).to(BF)
+    b.q[:] = 0.0
+    b.q[:, :, 7] = 3.0
+    c = P.PagedCache(b.k, b.v, means)
+    for budget in (1, blocks // 3, blocks - 5):
+        plan = P.PagedPlan(b.table, c, 1, 2, budget + 3)
+        lists = torch.zeros((1, 1, budget + 3), dtype=torch.int32, device=cuda)
+        plan.update(ids=b.tids)
+        c.select(b.q, plan, lists, sinks=1, window=2)
+        scores = means[pages[1:-2], 0, 7].float() * 3
+        want = torch.sort(torch.sort(scores, descending=True, stable=True).indices[:budget]).values + 1
+        assert lists[0, 0].tolist() == [0] + want.tolist() + [blocks - 2, blocks - 1]
 
 
 def test_lists_of_every_block_give_the_same_bits(cuda):

@@ -105,6 +105,16 @@ struct El<VIREO_PAGED_F16> {
     }
 };
 VH_DEV u32x4 ldu4(const void *p) { return *reinterpret_cast<const u32x4 *>(p); }
+// Inclusive prefix sums over the wave by DPP (row shifts, then the rows' totals carried on); every lane active.
+VH_DEV uint32_t wave_scan_u(uint32_t v) {
+    v += dpp_u<0x111>(v);
+    v += dpp_u<0x112>(v);
+    v += dpp_u<0x114>(v);
+    v += dpp_u<0x118>(v);
+    v += dpp_u<0x142, 0xA>(v);
+    v += dpp_u<0x143, 0xC>(v);
+    return v;
+}
 // with the non-temporal hint: what a launch reads once
 VH_DEV u32x4 ldu4_once(const void *p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)); }
 // 8 consecutive elements of a type known at run time (the same for the whole launch) as floats

@@ -18,9 +18,9 @@
 // and 16-bit matrix products that leave only the heads near the highest to fp64 33.9
 // (their operand reads 64 bytes of a key at a time).
 // choose_kernel: a workgroup per (sequence, kv head), its keys in registers,
-// finds the budget's lowest key by 8-bit digits of its distance from the lowest one
-// (two or three, where keys differ by their last bits four) and writes the blocks in
-// order by one prefix sum. Bound by its chain of loads, barriers and LDS atomics.
+// finds the budget's lowest score by a histogram of 256 bins of their range and the
+// ranks of the scores in its bin, and writes the blocks in order by one prefix sum.
+// Bound by its chain of loads, barriers and LDS atomics.
 #include <hip/hip_runtime.h>
 #include <errno.h>
 #include "paged.h"
@@ -29,7 +29,6 @@ namespace {
 
 constexpr int kScoreRows = 64;  // mean keys per workgroup of score_kernel
 constexpr int kHeads = 16;      // query heads in LDS at a time
-constexpr int kThreads = 1024;  // of choose_kernel
 
 struct SelectArgs {
     const uint16_t *means;
@@ -53,6 +52,10 @@ struct SelectArgs {
 VH_DEV uint32_t ordered(float f) {
     const uint32_t u = __float_as_uint(f + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+VH_DEV float score_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 // v of the lane 1 (xor) / 2 (xor) / 4 / 8 (rotated within 16) away
@@ -126,115 +129,147 @@ __global__ void __launch_bounds__(256) score_kernel(SelectArgs a) {
     if (sub < 4 && b + sub < hi) a.keys[(size_t(i) * a.n_kv + g) * a.max_blocks + b + sub] = ordered(float(best));
 }
 
-// Keys that a thread of choose_kernel holds in registers; a sequence with more
-// candidates reads them again in every pass.
-constexpr int kHeld = 8;
+// Keys of a bin that one wave ranks against each other; more are told apart by digits.
+constexpr uint32_t kFew = 64;
+// the most candidates of a sequence: 64 keys per thread of 1024
+constexpr int kMaxCandidates = 65536;
 
-__global__ void __launch_bounds__(kThreads) choose_kernel(SelectArgs a) {
-    __shared__ uint32_t hist[2][256], wlo[kThreads / 64], whi[kThreads / 64];
-    __shared__ uint64_t wsum[kThreads / 64];
-    __shared__ uint32_t found, left, there;
+// HELD: keys that a thread holds in registers (the host takes the fewest threads and
+// keys that hold every candidate). Straight code over them: a loop's keys from memory
+// or both forms of every pass took 7.4 us for 1 871 candidates, this 5.4.
+template <int NT, int HELD>
+__global__ void __launch_bounds__(NT) choose_kernel(SelectArgs a) {
+    __shared__ uint32_t hist[2][256], wlo[NT / 64], whi[NT / 64];
+    __shared__ uint2 wsum[NT / 64];
+    __shared__ uint32_t found, left, there, n_few, few[kFew];
     const int g = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int have = a.seqs[i].blocks;
     if (a.head->tag != a.tag) return;
     int32_t *list = a.lists + (size_t(i) * a.n_kv + g) * a.width;
     if (have <= a.width) {
-        for (int x = tid; x < a.width; x += kThreads) list[x] = x < have ? x : -1;
+        for (int x = tid; x < a.width; x += NT) list[x] = x < have ? x : -1;
         return;
     }
     const int budget = a.width - a.sinks - a.window, n = have - a.sinks - a.window;  // n > budget
     const uint32_t *keys = a.keys + (size_t(i) * a.n_kv + g) * a.max_blocks + a.sinks;
-    // thread tid's candidates: x0 .. x0 + per - 1 (below n), in order
-    const int per = (n + kThreads - 1) / kThreads, x0 = tid * per, cnt = max(min(per, n - x0), 0);
-    const bool held = per <= kHeld;
-    uint32_t k[kHeld];
+    // thread tid's candidates: x0 .. x0 + cnt - 1, in order
+    const int per = (n + NT - 1) / NT, x0 = tid * per, cnt = max(min(per, n - x0), 0);
+    uint32_t k[HELD];
 #pragma unroll
-    for (int j = 0; j < kHeld; j++) k[j] = held && j < cnt ? keys[x0 + j] : 0;
-    for (int x = tid; x < a.sinks; x += kThreads) list[x] = x;
-    for (int x = tid; x < a.window; x += kThreads) list[a.sinks + budget + x] = have - a.window + x;
+    for (int j = 0; j < HELD; j++) k[j] = j < cnt ? keys[x0 + j] : 0;  // no score's key is 0
+    for (int x = tid; x < a.sinks; x += NT) list[x] = x;
+    for (int x = tid; x < a.window; x += NT) list[a.sinks + budget + x] = have - a.window + x;
     if (budget == 0) return;
-    auto each = [&](auto f) {
-        if (held) {
-#pragma unroll
-            for (int j = 0; j < kHeld; j++)
-                if (j < cnt) f(x0 + j, k[j]);
-        } else {
-            for (int j = 0; j < cnt; j++) f(x0 + j, keys[x0 + j]);
-        }
-    };
-    // the range of the keys: digits are of key - lowest, so that they spread
+    // A bin of the scores' range that holds the budget's lowest: of 256 equal ones
+    // from the lowest score to the highest (digits of the keys would put scores of one
+    // exponent together). The bin of a score does not fall as the score rises: each step of
+    // its arithmetic is monotonous.
     uint32_t lo = 0xffffffffu, hi = 0;
-    each([&](int, uint32_t key) { lo = min(lo, key), hi = max(hi, key); });
+#pragma unroll
+    for (int j = 0; j < HELD; j++) lo = min(lo, k[j] - 1), hi = max(hi, k[j]);  // 0 - 1: not the lowest
     hi = wave_max_u(hi);
     lo = ~wave_max_u(~lo);
     if (lane == 0) wlo[wv] = lo, whi[wv] = hi;
-    if (tid < 512) hist[tid >> 8][tid & 255] = 0;
+    for (int x = tid; x < 512; x += NT) hist[x >> 8][x & 255] = 0;
+    if (tid == 0) n_few = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) lo = min(lo, wlo[w]), hi = max(hi, whi[w]);
-    // `need` of the keys whose (key - lo) >> shift is `top` are taken, and all above
-    int shift = 32 - __clz(hi - lo);  // __clz(0) is 32
-    uint32_t top = 0, need = uint32_t(budget);
-    for (int pass = 0; shift > 0; pass++) {
-        const int bits = min(shift, 8);
-        uint32_t *now = hist[pass & 1];
-        shift -= bits;
-        each([&](int, uint32_t key) {
-            const uint32_t v = (key - lo) >> shift;
-            if (uint64_t(v) >> bits == top) atomicAdd(&now[v & ((1u << bits) - 1)], 1u);
-        });
+    for (int w = 0; w < NT / 64; w++) lo = min(lo, wlo[w]), hi = max(hi, whi[w]);
+    const float flo = score_of(lo + 1), per_bin = 256.0f / (score_of(hi) - flo);
+    const bool even = per_bin > 0.0f && per_bin < INFINITY && flo > -INFINITY;  // else all in bin 0
+    auto bin_of = [&](uint32_t key) {
+        return key == 0 ? -1 : even ? min(int((score_of(key) - flo) * per_bin), 255) : 0;
+    };
+    // wave 0: the digit of `now`'s 256 that the need-th from the top falls into, to found, left, there
+    auto digit = [&](const uint32_t *now, uint32_t need) {
+        uint32_t c[4], sum = 0;  // lane l: 255 - 4 l .. 252 - 4 l
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum += c[j] = now[255 - 4 * lane - j];
+        uint32_t before = wave_scan_u(sum) - sum;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (before < need && before + c[j] >= need)
+                found = uint32_t(255 - 4 * lane - j), left = need - before, there = c[j];
+            before += c[j];
+        }
+    };
+    uint32_t need = uint32_t(budget);
+#pragma unroll
+    for (int j = 0; j < HELD; j++)
+        if (k[j]) atomicAdd(&hist[0][bin_of(k[j])], 1u);
+    __syncthreads();
+    if (wv == 0) digit(hist[0], need);
+    __syncthreads();
+    // the candidates of the bins above, and those of the bin itself
+    const int bin = int(found);
+    uint64_t above = 0, same = 0;
+#pragma unroll
+    for (int j = 0; j < HELD; j++) {
+        const int at = bin_of(k[j]);
+        above |= uint64_t(at > bin) << j;
+        same |= uint64_t(at == bin) << j;
+    }
+    // of the bin's keys, those above `least` are taken, and the first `need` of those equal to it
+    uint32_t least = 0;
+    need = left;
+    if (there == need) {
+        need = 0;  // all of them
+    } else if (there <= kFew) {
+#pragma unroll
+        for (int j = 0; j < HELD; j++)
+            if ((same >> j) & 1) few[atomicAdd(&n_few, 1u)] = k[j];
         __syncthreads();
-        if (wv == 0) {  // lane l: digits 255 - 4 l .. 252 - 4 l
-            uint32_t c[4], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) sum += c[j] = now[255 - 4 * lane - j];
-            uint32_t upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t u = __shfl_up(upto, o);
-                if (lane >= o) upto += u;
+        if (wv == 0) {
+            const int m = int(there);
+            const uint32_t mine = lane < m ? few[lane] : 0;
+            uint32_t gt = 0, ge = 0;
+            for (int j = 0; j < m; j++) {
+                const uint32_t o = uint32_t(__builtin_amdgcn_readlane(int(mine), j));
+                gt += o > mine, ge += o >= mine;
             }
-            uint32_t before = upto - sum;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (before < need && before + c[j] >= need)
-                    found = uint32_t(255 - 4 * lane - j), left = need - before, there = c[j];
-                before += c[j];
-            }
-        } else if (wv >= 4 && wv < 8) {
-            hist[(pass & 1) ^ 1][tid & 255] = 0;  // read last in the pass before
+            if (lane < m && gt < need && ge >= need) found = mine, left = need - gt;  // equal ones write the same
         }
         __syncthreads();
-        top = (top << bits) | found;
+        least = found;
         need = left;
-        if (there == need) break;  // all of them: the lower digits do not matter
-    }
-    // the keys above and the first `need` equal ones, in order: one prefix sum of both counts
-    uint32_t above = 0, equal = 0;
-    each([&](int, uint32_t key) {
-        const uint32_t v = uint32_t(uint64_t(key - lo) >> shift);
-        above += v > top, equal += v == top;
-    });
-    const uint64_t mine = (uint64_t(equal) << 32) | above;
-    uint64_t s = mine;
+    } else {  // digit by digit from the top
+        uint32_t top = 0;
+        for (int d = 24, pass = 1; d >= 0; d -= 8, pass++) {
+            uint32_t *now = hist[pass & 1];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t u = __shfl_up(s, o);
-        if (lane >= o) s += u;
+            for (int j = 0; j < HELD; j++)
+                if (((same >> j) & 1) && (d == 24 || k[j] >> (d + 8) == top)) atomicAdd(&now[(k[j] >> d) & 255], 1u);
+            __syncthreads();
+            if (wv == 0) digit(now, need);
+            else
+                for (int x = tid - 64; x < 256; x += NT - 64) hist[(pass & 1) ^ 1][x] = 0;  // read last in the pass before
+            __syncthreads();
+            top = (top << 8) | found;
+            need = left;
+        }
+        least = top;
     }
-    if (lane == 63) wsum[wv] = s;
+    // those taken, in order: one prefix sum of the ones above and of the equal ones
+    uint64_t equal = 0;
+#pragma unroll
+    for (int j = 0; j < HELD; j++) {
+        above |= uint64_t(((same >> j) & 1) && k[j] > least) << j;
+        equal |= uint64_t(((same >> j) & 1) && k[j] == least) << j;
+    }
+    const uint32_t na = __popcll(above), ne = __popcll(equal);
+    uint32_t gt = wave_scan_u(na), eq = wave_scan_u(ne);
+    if (lane == 63) wsum[wv] = make_uint2(gt, eq);
     __syncthreads();
-    uint64_t before = s - mine;
+    gt -= na, eq -= ne;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++)
-        if (w < wv) before += wsum[w];
-    uint32_t gt = uint32_t(before), eq = uint32_t(before >> 32);
-    each([&](int x, uint32_t key) {
-        const uint32_t v = uint32_t(uint64_t(key - lo) >> shift);
-        const bool take = v > top || (v == top && eq < need);
-        if (take) list[a.sinks + gt + min(eq, need)] = a.sinks + x;
-        gt += v > top, eq += v == top;
-    });
+    for (int w = 0; w < NT / 64; w++)
+        if (w < wv) gt += wsum[w].x, eq += wsum[w].y;
+    for (uint64_t m = above | equal; m; m &= m - 1) {
+        const int j = __builtin_ctzll(m);
+        const bool is_eq = (equal >> j) & 1;
+        if (!is_eq || eq < need) list[a.sinks + gt + min(eq, need)] = a.sinks + x0 + j;
+        gt += !is_eq, eq += is_eq;
+    }
 }
 
 }  // namespace
@@ -253,6 +288,7 @@ extern "C" int vireo_paged_select(const vireo_paged_cache *c, const vireo_paged_
                        p->table->max_blocks, v.head, v.seqs, v.tag, q, type, q_stride, p->n_heads / p->n_kv_heads, sinks,
                        window, p->list_blocks, v.keys, lists};
     const int cand = p->table->max_blocks - sinks - window;
+    if (cand > kMaxCandidates) return -E2BIG;
     if (p->table->max_blocks > p->list_blocks && p->list_blocks > sinks + window) {
         const dim3 grid(c->n_kv_heads, (cand + kScoreRows - 1) / kScoreRows, p->n);
         const bool bf = c->type == VIREO_PAGED_BF16;
@@ -266,6 +302,10 @@ extern "C" int vireo_paged_select(const vireo_paged_cache *c, const vireo_paged_
         SCORE(256)
 #undef SCORE
     }
-    hipLaunchKernelGGL(choose_kernel, dim3(c->n_kv_heads, p->n), dim3(kThreads), 0, s, a);
+    const dim3 lists_of(c->n_kv_heads, p->n);
+    if (cand <= 256 * 8) hipLaunchKernelGGL((choose_kernel<256, 8>), lists_of, dim3(256), 0, s, a);
+    else if (cand <= 512 * 8) hipLaunchKernelGGL((choose_kernel<512, 8>), lists_of, dim3(512), 0, s, a);
+    else if (cand <= 1024 * 8) hipLaunchKernelGGL((choose_kernel<1024, 8>), lists_of, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((choose_kernel<1024, 64>), lists_of, dim3(1024), 0, s, a);
     return vh_finish(s, vh_check(hipGetLastError()));
 }

@@ -13,10 +13,11 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
-// Rows that extend's one workgroup numbers itself (two per thread); more take
-// a second launch.
-constexpr int kRowsHere = 2048;
+constexpr int kThreads = 1024, kFewThreads = 256;  // a batch of at most kFewThreads takes so many: barriers of 4 waves
+// Rows that extend's one workgroup numbers itself, four per thread at a time; more
+// take a second launch over the chip (193 sequences, 4 558 rows: 4.5 and 6.3 us in two
+// launches, 7.9 in one).
+constexpr int kRowsHere = 8192;
 constexpr uint32_t kMaxRows = 0x7fffffff;
 
 VH_DEV int lane_id() { return threadIdx.x & 63; }
@@ -24,27 +25,28 @@ VH_DEV int lane_id() { return threadIdx.x & 63; }
 // Sums that stop at 2^31 - 1 (adding in any order gives the same).
 VH_DEV uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kMaxRows); }
 
-// Exclusive prefix sum over the workgroup's threads; *total receives the sum.
-// wsum: 16 words of LDS (two barriers inside; the caller's next use of wsum
-// comes after another one).
+// Exclusive prefix sum over the workgroup's NT threads; *total receives the sum.
+// wsum: a word of LDS per wave (one barrier inside; wsum is read after it, so
+// its next use needs another barrier in between).
+template <int NT>
 VH_DEV uint32_t block_scan(uint32_t v, uint32_t *wsum, uint32_t *total) {
     const int lane = lane_id(), wv = threadIdx.x >> 6;
     uint32_t s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t u = __shfl_up(s, o);
-        if (lane >= o) s = add_sat(s, u);
-    }
+    s = add_sat(s, dpp_u<0x111>(s));
+    s = add_sat(s, dpp_u<0x112>(s));
+    s = add_sat(s, dpp_u<0x114>(s));
+    s = add_sat(s, dpp_u<0x118>(s));
+    s = add_sat(s, dpp_u<0x142, 0xA>(s));
+    s = add_sat(s, dpp_u<0x143, 0xC>(s));
     if (lane == 63) wsum[wv] = s;
     __syncthreads();
     uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) {
+    for (int w = 0; w < NT / 64; w++) {
         const uint32_t u = wsum[w];
         before = w < wv ? add_sat(before, u) : before;
         all = add_sat(all, u);
     }
-    __syncthreads();
     *total = all;
     const uint32_t up = __shfl_up(s, 1);
     return add_sat(before, lane ? up : 0u);
@@ -79,10 +81,11 @@ __global__ void __launch_bounds__(256) reset_kernel(TableArgs t) {
 // The row of the table that batch entry i means, or -1 if it is out of range
 // or an earlier entry means it too. owner: LDS, max_seqs words; one barrier
 // before the answers.
+template <int NT>
 VH_DEV void claim(const int32_t *ids, int n, int max_seqs, int *owner) {
-    for (int s = threadIdx.x; s < max_seqs; s += kThreads) owner[s] = n;
+    for (int s = threadIdx.x; s < max_seqs; s += NT) owner[s] = n;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += NT) {
         const int id = ids ? ids[i] : i;
         if (id >= 0 && id < max_seqs) atomicMin(&owner[id], i);
     }
@@ -101,36 +104,57 @@ struct Seq {
     uint32_t off;      // blocks taken by earlier sequences
 };
 
-// position and slot of row r; blocks of before from the table, new ones from the stack below `top`
-VH_DEV void number_row(const TableArgs &t, const uint32_t *start, const Seq *seq, int n, int top, int r,
-                       int32_t *positions, int32_t *slots) {
-    int pos = 0, slot = -1;
-    if (uint32_t(r) < start[n]) {
-        const int i = find(start, n, uint32_t(r));
-        const Seq s = seq[i];
-        if (s.have >= 0) pos = int(s.base + (uint32_t(r) - start[i]));
-        if (s.row >= 0) {
-            const int b = pos >> t.shift;
-            const int blk = b < s.have ? t.blocks[size_t(s.row) * t.max_blocks + b]
-                                       : t.free_blocks[top - 1 - int(s.off + uint32_t(b - s.have))];
-            slot = (blk << t.shift) + (pos & ((1 << t.shift) - 1));
+// Positions and slots of rows r0, r0 + NT, ..., four at a time so that their loads
+// are in flight together; blocks of before from the table, new ones from the stack
+// below `top`.
+template <int NT>
+VH_DEV void number_rows(const TableArgs &t, const uint32_t *start, const Seq *seq, int n, int top, int max_rows,
+                        int32_t *positions, int32_t *slots) {
+    constexpr int U = 4;
+    const int mask = (1 << t.shift) - 1;
+    for (int r0 = threadIdx.x; r0 < max_rows; r0 += U * NT) {
+        int pos[U];
+        const int32_t *from[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t r = uint32_t(r0 + NT * u);
+            pos[u] = 0;
+            from[u] = nullptr;
+            if (r < start[n] && r < uint32_t(max_rows)) {
+                const int i = find(start, n, r);
+                const Seq s = seq[i];
+                if (s.have >= 0) pos[u] = int(s.base + (r - start[i]));
+                const int b = pos[u] >> t.shift;
+                if (s.row >= 0)
+                    from[u] = b < s.have ? t.blocks + size_t(s.row) * t.max_blocks + b
+                                         : t.free_blocks + (top - 1 - int(s.off + uint32_t(b - s.have)));
+            }
+        }
+        int blk[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) blk[u] = from[u] ? *from[u] : 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int r = r0 + NT * u;
+            if (r >= max_rows) break;
+            positions[r] = pos[u];
+            slots[r] = from[u] ? (blk[u] << t.shift) + (pos[u] & mask) : -1;
         }
     }
-    positions[r] = pos;
-    slots[r] = slot;
 }
 
 // One workgroup. Every entry's status, the prefix sums of rows and of blocks,
 // new table entries, lengths and the stack's height; then the rows' positions
 // and slots, if they are few (rows_here). LDS: owner [max_seqs], start [n + 1],
 // blocks' prefix sums [n + 1], Seq [n].
-__global__ void __launch_bounds__(kThreads) extend_kernel(TableArgs t, const int32_t *__restrict__ ids,
+template <int NT>
+__global__ void __launch_bounds__(NT) extend_kernel(TableArgs t, const int32_t *__restrict__ ids,
                                                           const int32_t *__restrict__ n_new, int n, int max_rows,
                                                           int32_t *__restrict__ start_out, int32_t *__restrict__ positions,
                                                           int32_t *__restrict__ slots, int32_t *__restrict__ status,
                                                           bool rows_here) {
     extern __shared__ uint32_t lds[];
-    __shared__ uint32_t wsum[2][kThreads / 64];
+    __shared__ uint32_t wsum[2][2][NT / 64];
     __shared__ uint32_t taken;
     int *owner = reinterpret_cast<int *>(lds);
     uint32_t *start = lds + t.max_seqs, *bsum = start + n + 1;
@@ -138,9 +162,9 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(TableArgs t, const int
     const int tid = threadIdx.x;
     const int n_free = min(max(*t.n_free, 0), t.n_blocks);
     if (tid == 0) taken = 0;
-    claim(ids, n, t.max_seqs, owner);
+    claim<NT>(ids, n, t.max_seqs, owner);
     uint32_t rows = 0, blocks = 0;  // of the chunks before
-    for (int c = 0; c < n; c += kThreads) {
+    for (int c = 0; c < n; c += NT) {
         const int i = c + tid;
         int row = -1, st = -EINVAL, need = 0, have = 0;
         uint32_t grow = 0, base = 0;
@@ -155,14 +179,14 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(TableArgs t, const int
             }
         }
         uint32_t all;
-        const uint32_t r0 = add_sat(rows, block_scan(grow, wsum[0], &all));
+        const uint32_t r0 = add_sat(rows, block_scan<NT>(grow, wsum[0][(c / NT) & 1], &all));
         rows = add_sat(rows, all);
         if (st == 0) {
             const uint32_t to = add_sat(base, grow);
             if (blocks_of(to, t.shift) > t.max_blocks || add_sat(r0, grow) > uint32_t(max_rows)) st = -E2BIG;
             else need = blocks_of(to, t.shift) - have;
         }
-        const uint32_t b0 = add_sat(blocks, block_scan(uint32_t(need), wsum[1], &all));
+        const uint32_t b0 = add_sat(blocks, block_scan<NT>(uint32_t(need), wsum[1][(c / NT) & 1], &all));
         blocks = add_sat(blocks, all);
         if (st == 0 && need > 0 && add_sat(b0, uint32_t(need)) > uint32_t(n_free)) st = -ENOSPC, need = 0;
         if (i < n) {
@@ -185,60 +209,58 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(TableArgs t, const int
     __syncthreads();
     if (tid == 0 && taken) *t.n_free = n_free - int(taken);
     // new table entries: the sequences that took blocks hold the first `taken` of the prefix sums
-    for (uint32_t b = tid; b < taken; b += kThreads) {
+    for (uint32_t b = tid; b < taken; b += NT) {
         const int i = find(bsum, n, b);
         const Seq s = seq[i];
         if (s.row >= 0)
             t.blocks[size_t(s.row) * t.max_blocks + s.have + int(b - s.off)] = t.free_blocks[n_free - 1 - int(b)];
     }
-    if (rows_here)
-        for (int r = tid; r < max_rows; r += kThreads) number_row(t, start, seq, n, n_free, r, positions, slots);
+    if (rows_here) number_rows<NT>(t, start, seq, n, n_free, max_rows, positions, slots);
 }
 
 // Positions and slots of many rows, after extend_kernel has filled the table.
 // Each workgroup has the batch's row numbers in LDS and takes kRowsPerGroup rows.
-constexpr int kRowsPerGroup = 1024;
-__global__ void __launch_bounds__(256) rows_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int max_rows,
+constexpr int kRowsPerGroup = 256;
+__global__ void __launch_bounds__(kRowsPerGroup) rows_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int max_rows,
                                                    const int32_t *__restrict__ start_in,
                                                    const int32_t *__restrict__ status, int32_t *__restrict__ positions,
                                                    int32_t *__restrict__ slots) {
     extern __shared__ uint32_t start[];
-    for (int i = threadIdx.x; i <= n; i += 256) start[i] = uint32_t(start_in[i]);
+    for (int i = threadIdx.x; i <= n; i += kRowsPerGroup) start[i] = uint32_t(start_in[i]);
     __syncthreads();
-    for (int k = 0; k < kRowsPerGroup; k += 256) {
-        const int r = blockIdx.x * kRowsPerGroup + k + threadIdx.x;
-        if (r >= max_rows) return;
-        int pos = 0, slot = -1;
-        if (uint32_t(r) < start[n]) {
-            const int i = find(start, n, uint32_t(r)), st = status[i];
-            if (st != -EINVAL) {  // a refused sequence's length is the one before
-                const int id = ids ? ids[i] : i;
-                pos = max(t.len[id], 0) - (st == 0 ? int(start[i + 1] - start[i]) : 0) + (r - int(start[i]));
-                if (st == 0)
-                    slot = (t.blocks[size_t(id) * t.max_blocks + (pos >> t.shift)] << t.shift) +
-                           (pos & ((1 << t.shift) - 1));
-            }
+    const int r = blockIdx.x * kRowsPerGroup + threadIdx.x;
+    if (r >= max_rows) return;
+    int pos = 0, slot = -1;
+    if (uint32_t(r) < start[n]) {
+        const int i = find(start, n, uint32_t(r)), st = status[i];
+        if (st != -EINVAL) {  // a refused sequence's length is the one before
+            const int id = ids ? ids[i] : i;
+            pos = max(t.len[id], 0) - (st == 0 ? int(start[i + 1] - start[i]) : 0) + (r - int(start[i]));
+            if (st == 0)
+                slot = (t.blocks[size_t(id) * t.max_blocks + (pos >> t.shift)] << t.shift) +
+                       (pos & ((1 << t.shift) - 1));
         }
-        positions[r] = pos;
-        slots[r] = slot;
     }
+    positions[r] = pos;
+    slots[r] = slot;
 }
 
 // One workgroup: the blocks that the batch's sequences give back, numbered in
 // the batch's order and in the order of positions, go on the stack in reverse
 // (the first on top). LDS: owner [max_seqs], prefix sums [n + 1], Seq [n].
-__global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const int32_t *__restrict__ ids,
+template <int NT>
+__global__ void __launch_bounds__(NT) truncate_kernel(TableArgs t, const int32_t *__restrict__ ids,
                                                             const int32_t *__restrict__ new_len, int n) {
     extern __shared__ uint32_t lds[];
-    __shared__ uint32_t wsum[kThreads / 64];
+    __shared__ uint32_t wsum[2][NT / 64];
     int *owner = reinterpret_cast<int *>(lds);
     uint32_t *bsum = lds + t.max_seqs;
     Seq *seq = reinterpret_cast<Seq *>(bsum + n + 1);
     const int tid = threadIdx.x;
     const int n_free = *t.n_free;
-    claim(ids, n, t.max_seqs, owner);
+    claim<NT>(ids, n, t.max_seqs, owner);
     uint32_t blocks = 0;
-    for (int c = 0; c < n; c += kThreads) {
+    for (int c = 0; c < n; c += NT) {
         const int i = c + tid;
         int row = -1, keep = 0, have = 0;
         if (i < n) {
@@ -254,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const i
             }
         }
         uint32_t all;
-        const uint32_t b0 = add_sat(blocks, block_scan(uint32_t(have - keep), wsum, &all));
+        const uint32_t b0 = add_sat(blocks, block_scan<NT>(uint32_t(have - keep), wsum[(c / NT) & 1], &all));
         blocks = add_sat(blocks, all);
         if (i < n) {
             bsum[i] = b0;
@@ -265,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const i
     __syncthreads();
     // a table that the caller filled may name blocks more often than there are any: the stack's end is its limit
     const int room = max(t.n_blocks - max(n_free, 0), 0), total = int(min(blocks, uint32_t(room)));
-    for (int b = tid; b < total; b += kThreads) {
+    for (int b = tid; b < total; b += NT) {
         const Seq s = seq[find(bsum, n, uint32_t(b))];
         t.free_blocks[max(n_free, 0) + total - 1 - b] =
             t.blocks[size_t(s.row) * t.max_blocks + s.have + (b - int(s.off))];
@@ -283,19 +305,21 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(TableArgs t, const i
 // tokens 408 and 353, 23 of 1 to 8 191 67 and 59. Between the two, 131 071 tokens take 113 at
 // 512, 121 at 1 024 and 162 at 4 096 workgroups, the 64 sequences 396, 364 and 354.
 // LDS: items' prefix sums [n + 1], tokens [n], rows [n].
-__global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int whole,
+template <int NT>
+__global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int whole,
                                                         int fine, int list_blocks, PlanHead *__restrict__ head,
                                                         PlanSeq *__restrict__ seqs,
                                                         int32_t *__restrict__ first, PlanItem *__restrict__ items,
                                                         uint32_t tag) {
     extern __shared__ uint32_t lds[];
-    __shared__ uint32_t wsum[2][kThreads / 64], many[3];
+    __shared__ uint32_t wsum[2][2][NT / 64], many[3];
     uint32_t *fst = lds, *tok = fst + n + 1;
     int *rw = reinterpret_cast<int *>(tok + n);
     const int tid = threadIdx.x;
     const uint32_t most = uint32_t(t.max_blocks) << t.shift;
+    if (tid < 3) many[tid] = 0;  // before the scan's barrier
     uint32_t total = 0;
-    for (int c = 0; c < n; c += kThreads) {
+    for (int c = 0; c < n; c += NT) {
         const int i = c + tid;
         uint32_t tokens = 0;
         if (i < n) {
@@ -309,19 +333,15 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
             seqs[i] = PlanSeq{rw[i], blocks};
         }
         uint32_t all;
-        block_scan((tokens + kPagedUnit - 1) / kPagedUnit, wsum[(c / kThreads) & 1], &all);
+        block_scan<NT>((tokens + kPagedUnit - 1) / kPagedUnit, wsum[0][(c / NT) & 1], &all);
         total = add_sat(total, all);
     }
     // the least S of three that gives at most `whole` items
-    if (tid < 3) many[tid] = 0;
-    __syncthreads();
     uint32_t tries[3], mine[3] = {};
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-        const uint64_t s16 = uint64_t(total) * (16 + k);
-        tries[k] = uint32_t(max((s16 + 16 * whole - 1) / (16 * whole), uint64_t(1)));
-    }
-    for (int i = tid; i < n; i += kThreads) {
+    tries[0] = max((total + whole - 1) / whole, 1u);
+    tries[1] = tries[0] + (tries[0] + 15) / 16;
+    tries[2] = tries[0] + (tries[0] + 7) / 8;
+    for (int i = tid; i < n; i += NT) {
         const uint32_t u = (tok[i] + kPagedUnit - 1) / kPagedUnit;
 #pragma unroll
         for (int k = 0; k < 3; k++) mine[k] += (u + tries[k] - 1) / tries[k];
@@ -335,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
     for (int k = 2; k >= 0; k--)
         if (many[k] <= uint32_t(whole)) S = tries[k];
     uint32_t sum = 0;
-    for (int c = 0; c < n; c += kThreads) {
+    for (int c = 0; c < n; c += NT) {
         const int i = c + tid;
         uint32_t k = 0;
         if (i < n) {
@@ -343,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
             if (m) k = (u + (u + m - 1) / m - 1) / ((u + m - 1) / m);  // items of ceil(u / m) units
         }
         uint32_t all;
-        const uint32_t f = sum + block_scan(k, wsum[(c / kThreads) & 1], &all);
+        const uint32_t f = sum + block_scan<NT>(k, wsum[1][(c / NT) & 1], &all);
         sum += all;
         if (i < n) {
             fst[i] = f;
@@ -357,7 +377,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(TableArgs t, const int32
         head->n_items = int32_t(sum);
     }
     __syncthreads();
-    for (uint32_t x = tid; x < sum; x += kThreads) {
+    for (uint32_t x = tid; x < sum; x += NT) {
         const int i = find(fst, n, x);
         const uint32_t k = fst[i + 1] - fst[i], u = (tok[i] + kPagedUnit - 1) / kPagedUnit, per = (u + k - 1) / k;
         const uint32_t b = (x - fst[i]) * per * kPagedUnit, e = min(b + per * kPagedUnit, tok[i]);
@@ -454,11 +474,16 @@ extern "C" int vireo_paged_extend(const vireo_paged_table *t, const int32_t *ids
     const TableArgs a = args_of(t);
     const bool here = max_rows <= kRowsHere;
     const size_t lds = 4 * size_t(t->max_seqs) + 8 * size_t(n + 1) + sizeof(Seq) * size_t(n);
-    if (int rc = allow_lds(extend_kernel, lds)) return rc;
-    hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(kThreads), lds, s, a, ids, n_new, n, max_rows, start, positions,
-                       slots, status, here);
+    if (n <= kFewThreads && max_rows <= kFewThreads && t->max_seqs <= kThreads) {
+        hipLaunchKernelGGL(extend_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), lds, s, a, ids, n_new, n, max_rows,
+                           start, positions, slots, status, here);
+    } else {
+        if (int rc = allow_lds(extend_kernel<kThreads>, lds)) return rc;
+        hipLaunchKernelGGL(extend_kernel<kThreads>, dim3(1), dim3(kThreads), lds, s, a, ids, n_new, n, max_rows, start,
+                           positions, slots, status, here);
+    }
     if (!here)
-        hipLaunchKernelGGL(rows_kernel, dim3((max_rows + kRowsPerGroup - 1) / kRowsPerGroup), dim3(256),
+        hipLaunchKernelGGL(rows_kernel, dim3((max_rows + kRowsPerGroup - 1) / kRowsPerGroup), dim3(kRowsPerGroup),
                            4 * size_t(n + 1), s, a, ids, n, max_rows, start, status, positions, slots);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
@@ -469,8 +494,12 @@ extern "C" int vireo_paged_truncate(const vireo_paged_table *t, const int32_t *i
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (n == 0) return vh_finish(s, 0);
     const size_t lds = 4 * size_t(t->max_seqs) + 4 * size_t(n + 1) + sizeof(Seq) * size_t(n);
-    if (int rc = allow_lds(truncate_kernel, lds)) return rc;
-    hipLaunchKernelGGL(truncate_kernel, dim3(1), dim3(kThreads), lds, s, args_of(t), ids, new_len, n);
+    if (n <= kFewThreads && t->max_seqs <= kThreads) {
+        hipLaunchKernelGGL(truncate_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), lds, s, args_of(t), ids, new_len, n);
+    } else {
+        if (int rc = allow_lds(truncate_kernel<kThreads>, lds)) return rc;
+        hipLaunchKernelGGL(truncate_kernel<kThreads>, dim3(1), dim3(kThreads), lds, s, args_of(t), ids, new_len, n);
+    }
     return vh_finish(s, vh_check(hipGetLastError()));
 }
 
@@ -484,7 +513,12 @@ extern "C" int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream) 
     hipStream_t s = static_cast<hipStream_t>(stream);
     const PlanView v = vh_plan_view(p);
     const size_t lds = 4 * size_t(p->n + 1) + 8 * size_t(p->n);
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n,
-                       plan_slots(p, kWholeGroups), plan_slots(p, kFineGroups), p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
+    const int whole = plan_slots(p, kWholeGroups), fine = plan_slots(p, kFineGroups);
+    if (p->n <= kFewThreads)
+        hipLaunchKernelGGL(plan_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), lds, s, args_of(p->table), p->ids, p->n,
+                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
+    else
+        hipLaunchKernelGGL(plan_kernel<kThreads>, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n,
+                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
