@@ -34,28 +34,28 @@ def _need(ok, what):
 
 
 def _ints(t, shape, dev, name):
-    """The address of a contiguous int32 tensor of this shape."""
-    if t.dtype is not _I32 or t.shape != shape or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous int32 tensor of shape {tuple(shape)} on {dev} is needed")
+    """The address of a contiguous int32 tensor of this shape; dev: the device's index."""
+    if t.dtype is not _I32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor of shape {tuple(shape)} on GPU {dev} is needed")
     return t.data_ptr()
 
 
 def _floats(t, n, dev, name):
-    if t is None:
-        return None
-    if t.dtype is not torch.float32 or t.numel() != n or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous float32 tensor of {n} values on {dev} is needed")
+    if t.dtype is not torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous float32 tensor of {n} values on GPU {dev} is needed")
     return t.data_ptr()
 
 
-def _rows(t, rows, heads, d, dev, name):
+def _rows(t, shape, dev, name):
     """Address, type and row stride of [rows, heads, d] rows whose heads are consecutive."""
-    if t.shape != (rows, heads, d) or t.device != dev or t.dtype not in _TYPES:
-        raise ValueError(f"{name}: a float32, float16 or bfloat16 tensor of shape {(rows, heads, d)} on {dev} is needed")
-    st = t.stride()
-    if (d > 1 and st[2] != 1) or (heads > 1 and st[1] != d):
+    kind = _TYPES.get(t.dtype)
+    if kind is None or t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{name}: a float32, float16 or bfloat16 tensor of shape {tuple(shape)} on GPU {dev} is needed")
+    rows, heads, d = shape
+    row, head, one = t.stride()
+    if one != 1 or (head != d and heads > 1):
         raise ValueError(f"{name}: the heads of a row have to be consecutive")
-    return t.data_ptr(), _TYPES[t.dtype], st[0] if rows > 1 else heads * d
+    return t.data_ptr(), kind, row if rows > 1 else heads * d
 
 
 class _On:
@@ -65,18 +65,19 @@ class _On:
         _need(device.type == "cuda", "a tensor on a GPU is needed")
         self.lib = _lib.load()
         self.device = device
+        self.index = device.index
 
     def call(self, name, stream, *args):
         fn = getattr(self.lib, name)
         if stream is None:
             stream = torch.cuda.current_stream(self.device)
-        elif stream.device != self.device:
+        elif stream.device_index != self.index:
             raise ValueError(f"a stream of {self.device} is needed")
-        if torch.cuda.current_device() != self.device.index:
+        if torch.cuda.current_device() == self.index:
+            rc = fn(*args, stream.cuda_stream)
+        else:
             with torch.cuda.device(self.device):
                 rc = fn(*args, stream.cuda_stream)
-        else:
-            rc = fn(*args, stream.cuda_stream)
         if rc:
             _lib.check(rc, name)
 
@@ -89,7 +90,8 @@ class PagedTable:
     def __init__(self, blocks, length, free_blocks, n_free, block_tokens):
         _need(blocks.dim() == 2 and free_blocks.dim() == 1, "blocks is [max_seqs, max_blocks], free_blocks [n_blocks]")
         self.on = _On(blocks.device)
-        self.device = dev = blocks.device
+        self.device = blocks.device
+        self.index = dev = blocks.get_device()
         self.max_seqs, self.max_blocks = blocks.shape
         self.n_blocks, self.block_tokens = free_blocks.numel(), block_tokens
         self.blocks, self.len, self.free_blocks, self.n_free = blocks, length, free_blocks, n_free
@@ -119,26 +121,24 @@ class PagedTable:
     def _ids(self, ids, n):
         if ids is None:
             return None
-        return _ints(ids, (n,), self.device, "ids")
+        return _ints(ids, (n,), self.index, "ids")
 
     def extend(self, n_new, start, positions, slots, status, ids=None, stream=None):
         """Room for n_new [n] more tokens (None: one each) of sequences ids [n] (None:
         0 .. n - 1): fills start [n + 1], positions and slots [max_rows] and status
         [n] (0 or a negative errno, per sequence: see the header)."""
-        n = status.numel()
+        n, rows, dev = status.numel(), slots.numel(), self.index
         self.on.call("vireo_paged_extend", stream, self._p, self._ids(ids, n),
-                     None if n_new is None else _ints(n_new, (n,), self.device, "n_new"), n, slots.numel(),
-                     _ints(start, (n + 1,), self.device, "start"),
-                     _ints(positions, (slots.numel(),), self.device, "positions"),
-                     _ints(slots, (slots.numel(),), self.device, "slots"),
-                     _ints(status, (n,), self.device, "status"))
+                     None if n_new is None else _ints(n_new, (n,), dev, "n_new"), n, rows,
+                     _ints(start, (n + 1,), dev, "start"), _ints(positions, (rows,), dev, "positions"),
+                     _ints(slots, (rows,), dev, "slots"), _ints(status, (n,), dev, "status"))
 
     def truncate(self, new_len=None, ids=None, stream=None):
         """Sequences ids cut back to new_len tokens (None: to none, which ends them);
         ids None: as many as new_len has, or every sequence."""
         n = ids.numel() if ids is not None else new_len.numel() if new_len is not None else self.max_seqs
         self.on.call("vireo_paged_truncate", stream, self._p, self._ids(ids, n),
-                     None if new_len is None else _ints(new_len, (n,), self.device, "new_len"), n)
+                     None if new_len is None else _ints(new_len, (n,), self.index, "new_len"), n)
 
 
 class PagedPlan:
@@ -151,6 +151,9 @@ class PagedPlan:
         self.table, self.n, self.n_heads, self.list_blocks = table, n, n_heads, list_blocks
         self.n_kv_heads, self.head_size = cache.n_kv_heads, cache.head_size
         self.ids = None
+        self._shape = (n, n_heads, cache.head_size)
+        self._lists = (n, cache.n_kv_heads, list_blocks)
+        self.index = table.index
         self.c = _lib.PagedPlanC(table._p, None, n, n_heads, cache.n_kv_heads, cache.head_size, list_blocks, None)
         self._p = C.pointer(self.c)
         nbytes = table.on.lib.vireo_paged_plan_bytes(self._p)
@@ -182,7 +185,7 @@ class PagedCache:
         _need(means is None or (means.shape == (nb, kv, d) and means.dtype is k.dtype and means.device == k.device and
                                 means.is_contiguous()), "means: [n_blocks, n_kv_heads, head_size] like k")
         self.on = _On(k.device)
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self.index = k.device, k.dtype, k.get_device()
         self.n_blocks, self.n_kv_heads, self.block_tokens, self.head_size = nb, kv, G, d
         self.k, self.v, self.means = k, v, means
         self.c = _lib.PagedCacheC(_TYPES[k.dtype], nb, G, kv, d, k.data_ptr(), v.data_ptr(),
@@ -204,35 +207,37 @@ class PagedCache:
         PagedTable.extend; norms and biases in fp32; rope: [max_pos, rotary] from
         vireo_rope_table (None: no rotation). q_out [T, n_heads, head_size] receives
         the queries for attend; k and v go into the cache."""
-        dev, d = self.device, self.head_size
+        dev, d, KV = self.index, self.head_size, self.n_kv_heads
         T, H = slots.numel(), q.shape[1]
-        qp, qt, qs = _rows(q, T, H, d, dev, "q")
-        kp, kt, ks = _rows(k, T, self.n_kv_heads, d, dev, "k")
-        vp, vt, vs = _rows(v, T, self.n_kv_heads, d, dev, "v")
-        op, ot, os_ = _rows(q_out, T, H, d, dev, "q_out")
+        qp, qt, qs = _rows(q, (T, H, d), dev, "q")
+        kp, kt, ks = _rows(k, (T, KV, d), dev, "k")
+        vp, vt, vs = _rows(v, (T, KV, d), dev, "v")
+        op, ot, os_ = _rows(q_out, (T, H, d), dev, "q_out")
         _need(qt == kt == vt, "q, k and v have to be of one type")
         max_pos, rotary = (0, 0) if rope is None else rope.shape
-        r = _lib.PagedRowsC(T, H, qt, qp, kp, vp, qs, ks, vs, _floats(q_bias, H * d, dev, "q_bias"),
-                            _floats(k_bias, self.n_kv_heads * d, dev, "k_bias"),
-                            _floats(v_bias, self.n_kv_heads * d, dev, "v_bias"), _floats(q_norm, d, dev, "q_norm"),
-                            _floats(k_norm, d, dev, "k_norm"), eps, _floats(rope, max_pos * rotary, dev, "rope"), rotary,
-                            max_pos, _ints(positions, (T,), dev, "positions"), _ints(slots, (T,), dev, "slots"), op, ot,
-                            os_)
+        r = _lib.PagedRowsC(T, H, qt, qp, kp, vp, qs, ks, vs,
+                            None if q_bias is None else _floats(q_bias, H * d, dev, "q_bias"),
+                            None if k_bias is None else _floats(k_bias, KV * d, dev, "k_bias"),
+                            None if v_bias is None else _floats(v_bias, KV * d, dev, "v_bias"),
+                            None if q_norm is None else _floats(q_norm, d, dev, "q_norm"),
+                            None if k_norm is None else _floats(k_norm, d, dev, "k_norm"), eps,
+                            None if rope is None else _floats(rope, max_pos * rotary, dev, "rope"), rotary, max_pos,
+                            _ints(positions, (T,), dev, "positions"), _ints(slots, (T,), dev, "slots"), op, ot, os_)
         self.on.call("vireo_paged_append", stream, self._p, C.byref(r))
 
     def _plan(self, plan):
-        _need(plan.table.device == self.device, f"a plan on {self.device} is needed")
+        _need(plan.index == self.index, f"a plan on {self.device} is needed")
         return plan._p
 
     def attend(self, q, out, plan, lists=None, scale=None, stream=None):
         """out [n, n_heads, head_size] = attention of q (one new token per sequence of
         the plan) over the sequences' blocks, or over lists [n, n_kv_heads,
         list_blocks] of them; scale: 1 / sqrt(head_size) if None."""
-        qp, qt, qs = _rows(q, plan.n, plan.n_heads, self.head_size, self.device, "q")
-        op, ot, os_ = _rows(out, plan.n, plan.n_heads, self.head_size, self.device, "out")
+        qp, qt, qs = _rows(q, plan._shape, self.index, "q")
+        op, ot, os_ = _rows(out, plan._shape, self.index, "out")
         _need(qt == ot, "q and out have to be of one type")
         _need((lists is not None) == (plan.list_blocks > 0), "lists go with a plan for lists, and only with one")
-        lp = None if lists is None else _ints(lists, (plan.n, plan.n_kv_heads, plan.list_blocks), self.device, "lists")
+        lp = None if lists is None else _ints(lists, plan._lists, self.index, "lists")
         self.on.call("vireo_paged_attend", stream, self._p, self._plan(plan), qp, qt, qs,
                      1.0 / math.sqrt(self.head_size) if scale is None else scale, lp, op, os_)
 
@@ -240,6 +245,6 @@ class PagedCache:
         """lists [n, n_kv_heads, plan.list_blocks]: the first `sinks` blocks of each
         sequence, its last `window` and the best of those between by mean key, in
         ascending order, -1 behind them."""
-        qp, qt, qs = _rows(q, plan.n, plan.n_heads, self.head_size, self.device, "q")
-        lp = _ints(lists, (plan.n, plan.n_kv_heads, plan.list_blocks), self.device, "lists")
+        qp, qt, qs = _rows(q, plan._shape, self.index, "q")
+        lp = _ints(lists, plan._lists, self.index, "lists")
         self.on.call("vireo_paged_select", stream, self._p, self._plan(plan), qp, qt, qs, sinks, window, lp)
