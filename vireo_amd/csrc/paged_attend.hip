@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     constexpr int QP = query_parts(QF);
     constexpr int WP = QF && T == VIREO_PAGED_BF16 ? 3 : 2;  // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
-    __shared__ __align__(16) float red[2][16][RS];
+    __shared__ __align__(16) float red[3][16][RS];
     __shared__ float2 wml[4][16];
     // heads vary fastest: a block's kv heads are neighbours in memory, and the
     // plan's unused items come last
@@ -263,21 +263,17 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     if (T == VIREO_PAGED_F16) f *= 0x1p-14f;
 #pragma unroll
     for (int d = 0; d < DT; d++) acc[d] *= f;
-    // sums of the four waves' outputs as (0 + 2) + (1 + 3)
+    // the first wave adds the others' outputs in order
+    if (wv > 0) {
 #pragma unroll
-    for (int half = 2; half >= 1; half--) {
-        if (wv >= half && wv < 2 * half) {
-#pragma unroll
-            for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(&red[wv - half][col][16 * d + 4 * grp]) = acc[d];
-        }
-        __syncthreads();
-        if (wv < half) {
-#pragma unroll
-            for (int d = 0; d < DT; d++) acc[d] += *reinterpret_cast<const f32x4 *>(&red[wv][col][16 * d + 4 * grp]);
-        }
-        __syncthreads();
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(&red[wv - 1][col][16 * d + 4 * grp]) = acc[d];
     }
+    __syncthreads();
     if (wv != 0 || col >= nh) return;
+#pragma unroll
+    for (int w = 0; w < 3; w++)
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d] += *reinterpret_cast<const f32x4 *>(&red[w][col][16 * d + 4 * grp]);
     const int h = h0 + col;
     if (it.seq < 0) {  // the sequence's only item
         const float inv = inverse(M, L);
