@@ -196,40 +196,55 @@ VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
 
 // A matrix operand of queries of type F32 (QF) or T as parts of T: lane (col,
 // grp) loads values 32 s + 0 .. 7 from element `at` on (its head's, 8 grp in) for
-// each step s. fp32 queries over fp16 are taken under a power of two that brings the
-// head's largest into [2^14, 2^15); returns its exponent.
-constexpr int query_parts(bool f32) { return f32 ? 3 : 1; }
+// each step s; load() only requests them, parts() waits. fp32 queries over fp16 are
+// taken under a power of two that brings the head's largest into [2^14, 2^15);
+// parts() returns its exponent.
 template <int D, uint32_t T, bool QF>
-VH_DEV int load_queries(const void *q, int64_t at, u32x4 (&w)[query_parts(QF)][D / 32]) {
-    constexpr int KS = D / 32;
-    if constexpr (!QF) {
-#pragma unroll
-        for (int s = 0; s < KS; s++) w[0][s] = ldu4(static_cast<const uint16_t *>(q) + at + 32 * s);
-        return 0;
-    } else {
-        float x[KS][8], big = 0.0f;
-        int e = 0;
+struct Queries {
+    static constexpr int KS = D / 32, P = QF ? 3 : 1;
+    u32x4 raw[KS][QF ? 2 : 1];
+    VH_DEV void load(const void *q, int64_t at) {
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            ld8(q, VIREO_PAGED_F32, at + 32 * s, x[s]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[s][j]));
+            if constexpr (QF) {
+                const float *p = static_cast<const float *>(q) + at + 32 * s;
+                raw[s][0] = ldu4(p);
+                raw[s][1] = ldu4(p + 4);
+            } else {
+                raw[s][0] = ldu4(static_cast<const uint16_t *>(q) + at + 32 * s);
+            }
         }
-        if constexpr (T == VIREO_PAGED_F16) {
-            big = head_max(big);
-            if (big > 0.0f && big < INFINITY) e = 14 - ilogbf(big);
+    }
+    VH_DEV int parts(u32x4 (&w)[P][KS]) const {
+        int e = 0;
+        if constexpr (!QF) {
+#pragma unroll
+            for (int s = 0; s < KS; s++) w[0][s] = raw[s][0];
+        } else {
+            float x[KS][8], big = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
-        }
+                for (int j = 0; j < 8; j++) {
+                    x[s][j] = __uint_as_float(raw[s][j >> 2][j & 3]);
+                    big = fmaxf(big, fabsf(x[s][j]));
+                }
+            if constexpr (T == VIREO_PAGED_F16) {
+                big = head_max(big);
+                if (big > 0.0f && big < INFINITY) e = 14 - ilogbf(big);
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            u32x4 p[3];
-            split8<T, 3>(x[s], p);
+                for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int k = 0; k < 3; k++) w[k][s] = p[k];
+                    for (int j = 0; j < 8; j++) x[s][j] = ldexpf(x[s][j], e);
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 p[3];
+                split8<T, 3>(x[s], p);
+#pragma unroll
+                for (int k = 0; k < 3; k++) w[k][s] = p[k];
+            }
         }
         return e;
     }
-}
+};

@@ -81,7 +81,7 @@ VH_DEV float inverse(float M, float L) {
 template <int D, uint32_t T, bool QF>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
     constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
-    constexpr int QP = query_parts(QF);
+    constexpr int QP = Queries<D, T, QF>::P;             // parts of a query
     constexpr int WP = QF && T == VIREO_PAGED_BF16 ? 3 : 2;  // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
     __shared__ __align__(16) float red[3][16][RS];
@@ -100,9 +100,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     const int shift = a.shift, G = 1 << shift;
 
     // the queries: column col's head, dimensions 32 s + 8 grp .. + 7 of step s
-    u32x4 qw[QP][KS];
-    const int e = load_queries<D, T, QF>(a.q, seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp, qw);
-    const float c = ldexpf(ldexpf(a.c, -(e / 2)), e / 2 - e);  // in two steps: 2^e alone may leave fp32's range
+    // (formed below, once the first keys and values are requested too)
+    Queries<D, T, QF> query;
+    query.load(a.q, seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp);
 
     // the wave's tiles, and the blocks behind them, 64 at a time: lane e holds
     // block e0 + e of the sequence (or of its list) and how many of its slots
@@ -175,11 +175,15 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     f32x4 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    blocks_from((it.begin + 32 * i0) >> shift);
+    Where w = where(i0);  // i0 < T0; a wave without tiles reads one that it does not use
+    load_k(w);
+    load_v(w);
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 qw[QP][KS];
+    const int e = query.parts(qw);
+    const float c = ldexpf(ldexpf(a.c, -(e / 2)), e / 2 - e);  // in two steps: 2^e alone may leave fp32's range
     if (i0 < i1) {
-        blocks_from((it.begin + 32 * i0) >> shift);
-        Where w = where(i0);
-        load_k(w);
-        load_v(w);
         for (int i = i0; i < i1; i++) {
             f32x4 s[2];
 #pragma unroll
