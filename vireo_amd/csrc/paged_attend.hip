@@ -23,7 +23,8 @@
 // soon as the scores are formed and values as soon as they are weighed, so a
 // wave has a tile of 64 hs bytes in flight nearly all the time. They are read
 // once, with the non-temporal hint: 64 sequences of 500 to 30 001 tokens (1.9 GB)
-// 343 -> 318 us, 5.9 TB/s. Bound by that read; the matrix cores take a tenth of
+// 343 -> 318 us, 5.9 TB/s - but for the values of blocks of 64 slots and more, whose lines
+// two tiles share (16 sequences, 275 MB: 78 us with the hint, 67 without; 60 in blocks of 16 and 32). Bound by that read; the matrix cores take a tenth of
 // the time even with fp32 queries and weights in three parts each.
 //
 // Precision: products of 16-bit parts are exact in the matrix cores and their
@@ -77,8 +78,9 @@ VH_DEV float inverse(float M, float L) {
     return M == -INFINITY ? 0.0f : L == 0.0f ? __builtin_nanf("") : 1.0f / L;
 }
 
-// D: head size; T: the cache's type; QF: fp32 queries and results (else T's)
-template <int D, uint32_t T, bool QF>
+// D: head size; T: the cache's type; QF: fp32 queries and results (else T's);
+// ONCE: blocks of 16 or 32 slots, whose lines of values belong to one tile
+template <int D, uint32_t T, bool QF, bool ONCE>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
     constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
     constexpr int QP = Queries<D, T, QF>::P;             // parts of a query
@@ -167,7 +169,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
         const int off = (grp >> 1 ? w.off[1] : w.off[0]) + 8 * (grp & 1);
         const uint16_t *p = a.v + base + (size_t(col) << shift) + off;
 #pragma unroll
-        for (int d = 0; d < DT; d++) vv[d] = ldu4_once(p + (size_t(16 * d) << shift));
+        for (int d = 0; d < DT; d++) {
+            const uint16_t *pd = p + (size_t(16 * d) << shift);
+            vv[d] = ONCE ? ldu4_once(pd) : ldu4(pd);
+        }
     };
 
     float m = kLowest, l = 0.0f;
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
 // item i (256 at a time), groups of D / 4 threads take every NG-th item, four
 // dimensions a thread, and are added in order. The first NG U items' outputs are
 // requested with the weights' inputs, not after them. One thread per item's
-// maximum in turn took 66 us for 256 items of 32 heads, this 6.
+// maximum in turn took 66 us for 256 items of 32 heads, this 6.7 (4.7 for 64).
 template <int D, uint32_t T, bool QF>
 __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
     constexpr int ND = D / 4, NG = 256 / ND, U = 8;
@@ -373,7 +378,9 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
 
 template <int D, uint32_t T, bool QF>
 void launch_attend(const AttendArgs &a, int cap, int n, hipStream_t s) {
-    hipLaunchKernelGGL((attend_kernel<D, T, QF>), dim3(a.n_kv * a.tiles, cap), dim3(256), 0, s, a);
+    const dim3 grid(a.n_kv * a.tiles, cap);
+    if (a.shift < 6) hipLaunchKernelGGL((attend_kernel<D, T, QF, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<D, T, QF, false>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
 }
 
