@@ -165,7 +165,7 @@ int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream);
 /* out_i = softmax(scale q_i . K) V over sequence i's tokens, its newest among
  * them (extend and append come first): q, out [n x n_heads x head_size], rows
  * q_stride / out_stride elements apart, of `type` (F32 or the cache's), 16-byte
- * aligned. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
+ * aligned. out may be q. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
  * are in fp32 or exact: fp32 queries are split into three 16-bit parts, and weights into
  * as many as the output's type needs.
  * lists (NULL unless p->list_blocks > 0): [n x n_kv_heads x list_blocks], for

@@ -103,10 +103,11 @@ def half_step(dtype):
 
 
 def attend_bound(out64, weight64, size, d, dtype, cache):
-    """How far an output may be from fp64: the result's rounding; its weights' truncation to 16 bits (bf16) or 22
-    (fp16), or 24 (fp32 results over bf16); and the scores' fp32 sums, each of at most 32 terms inside the matrix cores
+    """How far an output may be from fp64: the result's rounding; its weights' truncation to 16 bits (bf16: what is cut
+    off is less than 2^-15 of the leading bit) or 22 (fp16: less than 2^-21), none where the result is fp32 (three
+    parts hold all 24 bits); and the scores' fp32 sums, each of at most 32 terms inside the matrix cores
     and d / 32 steps of at most 3 parts, whose relative error in units of 2^-24 goes into every weight twice (it and
     the sum), with 16 for the exponential, the scale and the sums over tokens."""
     u = 2.0 ** -24
-    cut = 2.0 ** -22 if cache is torch.float16 else 2.0 ** -15 if dtype is not torch.float32 else 2.0 ** -23
+    cut = 0.0 if dtype is torch.float32 else 2.0 ** -15 if cache is torch.bfloat16 else 2.0 ** -21
     return half_step(dtype) * out64.abs() + weight64 * (cut + 2 * u * ((32 + 3 * d // 32) * size + 16))

@@ -212,6 +212,30 @@ def test_append(cuda, d, H, KV, G, tin, tc, tq, rotary, norms, biases, T):
         assert torch.equal(ik, gk) and torch.equal(iv, gv) and torch.equal(q[live], out[live])
 
 
+def test_append_of_no_rows_and_of_weights_anywhere(cuda):
+    """A step without rows changes nothing; norm weights, biases and the rotation's table at any 4-byte address; rows of
+    a wider projection."""
+    d, H, KV, G, T = 128, 4, 2, 16, 5
+    k, v = (torch.zeros(s, dtype=BF, device=cuda) for s in ((4, KV, G, d), (4, KV, d, G)))
+    cache = P.PagedCache(k, v, torch.zeros((4, KV, d), dtype=BF, device=cuda))
+    none = torch.zeros(0, dtype=torch.int32, device=cuda)
+    x0 = torch.zeros((0, H + 2 * KV, d), dtype=F32, device=cuda)
+    cache.append(x0[:, :H], x0[:, H:H + KV], x0[:, H + KV:], none, none, torch.zeros((0, H, d), device=cuda))
+    assert torch.count_nonzero(k) == 0
+    x = torch.randn((T, 64 + (H + 2 * KV) * d + 4), generator=gen(cuda, 1), device=cuda)[:, 64:-4].unflatten(1, (-1, d))
+    pool = torch.randn(1 + d + d + H * d + 40 * d, generator=gen(cuda, 2), device=cuda)
+    qn, kn, qb, rope = (t.clone() for t in (pool[1:1 + d], pool[1 + d:1 + 2 * d], pool[1 + 2 * d:1 + 2 * d + H * d],
+                                            pool[-40 * d:].view(40, d)))
+    odd = lambda t: torch.cat([pool[:1], t.reshape(-1)])[1:].view(t.shape)  # noqa: E731  4 bytes off 16
+    pos, slots = ints([3, 0, 39, 7, 1], cuda), ints([17, 16, 63, 0, 5], cuda)
+    outs = []
+    for f in (lambda t: t, odd):
+        out = torch.zeros((T, H, d), device=cuda)
+        cache.append(x[:, :H], x[:, H:H + KV], x[:, H + KV:], pos, slots, out, f(rope), f(qn), f(kn), q_bias=f(qb))
+        outs.append((out, k.clone(), v.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 # ---- attention ------------------------------------------------------------------------------------------------------
 
 class Batch:
@@ -254,8 +278,8 @@ class Batch:
         self.cache.attend(self.q, out, plan, lists=lists, scale=scale, stream=stream)
         return out
 
-    def check(self, out, scale=None, chosen=None):
-        """Each output within its bound; chosen(i, g): (blocks of the sequence, attended slots of each) or None for all."""
+    def check(self, out, scale=None, chosen=None, more=0.0):
+        """Each output within its bound, and `more`; chosen(i, g): (blocks of the sequence, attended slots of each) or None for all."""
         scale = 1 / math.sqrt(self.d) if scale is None else scale
         group, worst = self.H // self.KV, 0.0
         for i, t in enumerate(self.lens):
@@ -264,7 +288,7 @@ class Batch:
                 take = chosen(i, g) if chosen else [(b, min(self.G, t - b * self.G)) for b in range(-(-t // self.G))]
                 ref, wt, size = attend64(self.q[i, h], self.k[:, g], self.v[:, g],
                                          [self.rows[self.ids[i]][b] for b, _ in take], [m for _, m in take], scale)
-                bound = attend_bound(ref, wt, size, self.d, out.dtype, self.cache.dtype)
+                bound = attend_bound(ref, wt, size, self.d, out.dtype, self.cache.dtype) + more
                 err = (out[i, h].double() - ref).abs()
                 assert bool((err <= bound).all()), (i, g, t, float(err.max()), float((err / bound.clamp(min=1e-30)).max()))
                 if bound.numel() and float(bound.max()) > 0:
@@ -379,6 +403,31 @@ def test_fp32_queries_of_any_size_over_fp16(cuda, magnitude):
     b.q *= magnitude
     scale = 1 / (magnitude * math.sqrt(128))
     b.check(b.attend(scale=scale), scale=scale)
+
+
+def test_small_keys_and_values_of_fp16(cuda):
+    """Keys and values far below fp16's least normal value (2^-14) are not flushed, and their outputs are as near as if
+    they were 2^-14: a subnormal's exponent field is that of 2^-14, the matrix cores align the 32 products of a
+    sum (weights of up to 2^14 times 2^-14) by these fields and cut off what lies 24 bits below, 2^-24 for each of three parts
+    and as much for the sum they are added to, 8 2^-24 with the sums' own rounding; the sum of the weights is at least 2^14."""
+    b = Batch(cuda, [300, 65, 1], 8, 2, 128, 16, HF, F32, seed=18)
+    b.k *= 2.0 ** -16
+    b.v *= 2.0 ** -18
+    b.q *= 2.0 ** 16
+    for t in (b.k, b.v):  # the junk of unwritten slots may have become finite: it stays unread
+        t[torch.isnan(t)] = math.inf
+    b.check(b.attend(), more=8 * 2.0 ** -38)
+
+
+@pytest.mark.parametrize("query", [BF, F32])
+def test_output_over_the_queries(cuda, query):
+    """out may be q itself."""
+    b = Batch(cuda, [3000, 0, 1, 700], 8, 2, 128, 16, BF, query, seed=19)
+    want = b.attend()
+    plan = P.PagedPlan(b.table, b.cache, 4, 8)
+    plan.update(ids=b.tids)
+    b.cache.attend(b.q, b.q, plan)
+    assert torch.equal(b.q, want)
 
 
 def test_bad_table_entries_are_skipped(cuda):

@@ -205,6 +205,7 @@ void launch_append(AppendArgs a, uint16_t *means, hipStream_t s) {
 extern "C" int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_rows *r, void *stream) {
     if (!vh_cache_ok(c) || !r || r->rows < 0 || r->n_heads < 1 || r->n_heads > 65535) return -EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (r->rows == 0) return vh_finish(s, 0);
     const int hs = c->head_size;
     if (!vh_rows_ok(r->q, r->type, r->q_stride, r->n_heads, hs, r->rows) ||
         !vh_rows_ok(r->k, r->type, r->k_stride, c->n_kv_heads, hs, r->rows) ||
@@ -216,7 +217,6 @@ extern "C" int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_
         return -EINVAL;
     const int64_t heads = int64_t(r->rows) * (r->n_heads + 2 * int64_t(c->n_kv_heads));
     if (heads > (int64_t(1) << 31)) return -E2BIG;
-    if (r->rows == 0) return vh_finish(s, 0);
     int shift = 4;
     while ((1 << shift) < c->block_tokens) shift++;
     const AppendArgs a{*r, static_cast<uint16_t *>(c->k), static_cast<uint16_t *>(c->v), c->type, c->n_kv_heads, shift,

@@ -28,12 +28,14 @@
 // the time even with fp32 queries and weights in three parts each.
 //
 // Precision: products of 16-bit parts are exact in the matrix cores and their
-// sums fp32. An fp32 query is the sum of three truncated 16-bit parts (bf16: 24
-// bits; fp16, under a power of two per head: 33 bits), a weight of two (bf16: 16
-// bits, far below the half step 2^-9 of a 16-bit result) or, for fp32 results,
-// three (24 bits) in bf16 and two (22 bits) in fp16. The sum of weights is of
-// the fp32 values. Parts that would be zero get the least value of the query's
-// sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
+// sums fp32 (fp16 values below 2^-14 are not flushed, but their products are added
+// as if they were that large: absolute errors of 2^-38 of the largest weight). An fp32
+// query is the sum of three truncated 16-bit parts (fp16: under a power of two per
+// head), and so is a weight for an fp32 result: every bit of them. For a 16-bit
+// result a weight is two parts: 16 bits in bf16, 22 in fp16, with errors under 2^-15
+// and 2^-21 against the result's half step of 2^-8 and 2^-11. The sum of weights is
+// of the fp32 values. Parts that would be zero get the least value of the
+// query's sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
 //
 // Waves merge through LDS, items in a second launch (merge_kernel) in the
 // items' order: the same bits every time. A sequence of one item is written by
@@ -84,7 +86,7 @@ template <int D, uint32_t T, bool QF, bool ONCE>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
     constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
     constexpr int QP = Queries<D, T, QF>::P;             // parts of a query
-    constexpr int WP = QF && T == VIREO_PAGED_BF16 ? 3 : 2;  // parts of a weight
+    constexpr int WP = QF ? 3 : 2;                       // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
     __shared__ __align__(16) float red[3][16][RS];
     __shared__ float2 wml[4][16];
