@@ -325,6 +325,29 @@ def test_attend_long(cuda, d, H, KV, G, cache, query, lens):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("d,H,KV,query", [(128, 32, 4, BF), (64, 16, 16, BF), (256, 32, 2, F32)])
+def test_repeated_calls_join_their_own_partials(cuda, d, H, KV, query):
+    """Two batches of queries in turn over one plan whose items the last workgroup joins: every call gives the first
+    call's bits, not what an earlier call left in the plan's memory."""
+    b = Batch(cuda, [1500, 1000, 0, 129, 257] if d < 256 else [900, 129, 0, 128, 257], H, KV, d, 16, BF, query, seed=20)
+    plan = P.PagedPlan(b.table, b.cache, 5, H)
+    plan.update(ids=b.tids)
+    qs = [b.q, (b.q * 0.5).contiguous()]
+    first = [torch.empty_like(b.q) for _ in qs]
+    for q, o in zip(qs, first):
+        b.cache.attend(q, o, plan)
+    b.check(first[0])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = [torch.empty((40, *b.q.shape), dtype=query, device=cuda) for _ in qs]
+    for i in range(40):
+        for q, o in zip(qs, outs):
+            b.cache.attend(q, o[i], plan, stream=stream)
+    torch.cuda.synchronize()
+    for o, f in zip(outs, first):
+        assert bool((o == f).all())
+
+
 def test_attend_many_short(cuda):
     lens = [random.Random(1).randint(0, 40) for _ in range(700)]
     b = Batch(cuda, lens, 4, 2, 64, 16, BF, BF, seed=4)

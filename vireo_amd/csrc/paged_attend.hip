@@ -37,10 +37,12 @@
 // of the fp32 values. Parts that would be zero get the least value of the
 // query's sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
 //
-// Waves merge through LDS, items in a second launch (merge_kernel) in the
-// items' order: the same bits every time. A sequence of one item is written by
-// the first launch. (A merge by the last workgroup to arrive needs its release
-// fence to write back the L2, which costs more than the launch.)
+// Waves merge through LDS. A sequence of one item is then written; others' partial
+// results are joined in the items' order, so that the bits are the same every time:
+// by a second launch (merge_kernel), or, where a sequence can have but few units
+// (short tables and lists of blocks: paged.h), by the last workgroup to arrive. Its inputs are stored and loaded past the dies' L2s (sc1), each store
+// completed before its workgroup counts as arrived: a release fence instead would write back
+// the L2, which costs more than the launch.
 #include <hip/hip_runtime.h>
 #include <errno.h>
 #include "paged.h"
@@ -70,6 +72,7 @@ struct AttendArgs {
     uint32_t tag;
     float *part;
     float2 *ml;
+    uint32_t *arrivals;  // or null: merge_kernel joins the items
 };
 
 // the wave's value of lane l's v (l the same on every lane)
@@ -78,6 +81,15 @@ VH_DEV int at_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 // score -inf (no weight at all), a NaN, as the softmax of them is.
 VH_DEV float inverse(float M, float L) {
     return M == -INFINITY ? 0.0f : L == 0.0f ? __builtin_nanf("") : 1.0f / L;
+}
+
+// four results
+template <uint32_t T, bool QF>
+VH_DEV void store4(void *out, int64_t at, f32x4 y) {
+    if constexpr (QF)
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(out) + at) = y;
+    else
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + at) = u32x2{El<T>::pack(y[0], y[1]), El<T>::pack(y[2], y[3])};
 }
 
 // D: head size; T: the cache's type; QF: fp32 queries and results (else T's);
@@ -100,7 +112,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int g = hg / a.tiles, z = hg - g * a.tiles;
-    const int seq = it.seq & 0x7fffffff, h0 = g * a.hpg + z * 16, nh = min(16, a.hpg - z * 16);
+    const int seq = it.seq, h0 = g * a.hpg + z * 16, nh = min(16, a.hpg - z * 16);
     const int shift = a.shift, G = 1 << shift;
 
     // the queries: column col's head, dimensions 32 s + 8 grp .. + 7 of step s
@@ -280,33 +292,93 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
         for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(&red[wv - 1][col][16 * d + 4 * grp]) = acc[d];
     }
     __syncthreads();
-    if (wv != 0 || col >= nh) return;
+    // partials of the sequence's items, for this tile's first head; at most kJoinUnits items where they are joined here
+    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
+        a.part + (size_t(it.first) * a.n_heads + h0) * D, 0, int(uint32_t(it.count * a.n_heads - h0) * D * 4u), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc(
+        a.ml + size_t(it.first) * a.n_heads + h0, 0, (it.count * a.n_heads - h0) * 8, 0x00020000);
+    const int64_t o0 = seq * a.out_stride + int64_t(h0) * D;
+    if (wv == 0 && col < nh) {
 #pragma unroll
-    for (int w = 0; w < 3; w++)
+        for (int w = 0; w < 3; w++)
 #pragma unroll
-        for (int d = 0; d < DT; d++) acc[d] += *reinterpret_cast<const f32x4 *>(&red[w][col][16 * d + 4 * grp]);
-    const int h = h0 + col;
-    if (it.seq < 0) {  // the sequence's only item
-        const float inv = inverse(M, L);
-        const int64_t o = seq * a.out_stride + int64_t(h) * D + 4 * grp;
+            for (int d = 0; d < DT; d++) acc[d] += *reinterpret_cast<const f32x4 *>(&red[w][col][16 * d + 4 * grp]);
+        if (it.count == 1) {
+            const float inv = inverse(M, L);
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const f32x4 y = acc[d] * inv;
-            if constexpr (QF) {
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + o + 16 * d) = y;
-            } else {
-                u32x2 w;
-                w[0] = El<T>::pack(y[0], y[1]);
-                w[1] = El<T>::pack(y[2], y[3]);
-                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + o + 16 * d) = w;
+            for (int d = 0; d < DT; d++) store4<T, QF>(a.out, o0 + col * D + 16 * d + 4 * grp, acc[d] * inv);
+        } else if (a.arrivals) {  // past the L2 of this die, which others do not keep coherent (sc1)
+            const int at = (item - it.first) * a.n_heads + col;
+            if (grp == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, rm, at * 8, 0, 16);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[d]), rp,
+                                                       (at * D + 16 * d + 4 * grp) * 4, 0, 16);
+        } else {
+            const size_t ph = size_t(item) * a.n_heads + h0 + col;
+            if (grp == 0) a.ml[ph] = make_float2(M, L);
+#pragma unroll
+            for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(a.part + ph * D + 16 * d + 4 * grp) = acc[d];
+        }
+    }
+    if (it.count == 1 || !a.arrivals) return;
+    // The last of the sequence's items to arrive joins them all, in their order.
+    __shared__ int last;
+    if (wv == 0) {
+        __builtin_amdgcn_s_waitcnt(0);  // the stores above have completed
+        asm volatile("" ::: "memory");
+        if (lane == 0) {
+            uint32_t *arrived = a.arrivals + size_t(seq) * gridDim.x + hg;
+            last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(it.count - 1);
+            if (last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    // D / 4 threads a head, HT heads a thread, U items of each at a time: 8 heads of at most U items in one go
+    constexpr int ND = D / 4, NG = 256 / ND, HT = D <= 128 ? 1 : 2, U = D <= 128 ? 8 : 16;
+    const int dq = threadIdx.x % ND;
+    for (int h = threadIdx.x / ND; h < nh; h += HT * NG) {
+        float m1[HT], l1[HT];
+        f32x4 y[HT];
+#pragma unroll
+        for (int x = 0; x < HT; x++) m1[x] = -INFINITY, l1[x] = 0.0f, y[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < it.count; i0 += U) {
+            u32x2 ml[HT][U];
+            u32x4 v[HT][U];
+#pragma unroll
+            for (int x = 0; x < HT; x++)
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int at = min(i0 + u, it.count - 1) * a.n_heads + min(h + NG * x, nh - 1);
+                    ml[x][u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, at * 8, 0, 16));
+                    v[x][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (at * D + 4 * dq) * 4, 0, 16));
+                }
+#pragma unroll
+            for (int x = 0; x < HT; x++) {
+                float big = m1[x];
+#pragma unroll
+                for (int u = 0; u < U; u++) big = fmaxf(big, __uint_as_float(ml[x][u][0]));  // repeats of the last one too
+                if (big == -INFINITY) continue;
+                const float back = __builtin_amdgcn_exp2f(m1[x] - big);
+                l1[x] *= back;
+                y[x] *= back;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (i0 + u < it.count) {
+                        const float f1 = __builtin_amdgcn_exp2f(__uint_as_float(ml[x][u][0]) - big);
+                        l1[x] = fmaf(__uint_as_float(ml[x][u][1]), f1, l1[x]);
+                        y[x] += __builtin_bit_cast(f32x4, v[x][u]) * f1;
+                    }
+                m1[x] = big;
             }
         }
-        return;
-    }
-    const size_t ph = size_t(item) * a.n_heads + h;
-    if (grp == 0) a.ml[ph] = make_float2(M, L);
 #pragma unroll
-    for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4 *>(a.part + ph * D + 16 * d + 4 * grp) = acc[d];
+        for (int x = 0; x < HT; x++)
+            if (h + NG * x < nh)
+                store4<T, QF>(a.out, o0 + (h + NG * x) * D + 4 * dq, y[x] * inverse(m1[x], l1[x]));
+    }
 }
 
 // A workgroup per (sequence, head) joins its items: thread i forms the weight of
@@ -366,16 +438,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
     if (grp) return;
 #pragma unroll
     for (int u = 1; u < NG; u++) y += red[u][dq];
-    y *= inverse(M, L);
-    const int64_t o = seq * a.out_stride + int64_t(h) * D + 4 * dq;
-    if constexpr (QF) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + o) = y;
-    } else {
-        u32x2 w;
-        w[0] = El<T>::pack(y[0], y[1]);
-        w[1] = El<T>::pack(y[2], y[3]);
-        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + o) = w;
-    }
+    store4<T, QF>(a.out, seq * a.out_stride + int64_t(h) * D + 4 * dq, y * inverse(M, L));
 }
 
 template <int D, uint32_t T, bool QF>
@@ -383,7 +446,7 @@ void launch_attend(const AttendArgs &a, int cap, int n, hipStream_t s) {
     const dim3 grid(a.n_kv * a.tiles, cap);
     if (a.shift < 6) hipLaunchKernelGGL((attend_kernel<D, T, QF, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attend_kernel<D, T, QF, false>), grid, dim3(256), 0, s, a);
-    hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
+    if (!a.arrivals) hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
 }
 
 template <int D>
@@ -414,7 +477,7 @@ extern "C" int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_
     const AttendArgs a{static_cast<const uint16_t *>(c->k), static_cast<const uint16_t *>(c->v), c->n_blocks,
                        c->n_kv_heads, shift, p->table->blocks, p->table->len, p->table->max_blocks, lists,
                        p->list_blocks, q, q_stride, scale * kLog2e, p->n_heads, p->n_heads / p->n_kv_heads,
-                       vh_plan_head_tiles(p), out, out_stride, type, v.head, v.items, v.first, v.tag, v.part, v.ml};
+                       vh_plan_head_tiles(p), out, out_stride, type, v.head, v.items, v.first, v.tag, v.part, v.ml, v.arrivals};
     if (c->head_size == 64) launch_types<64>(c->type, a, v.cap, p->n, s);
     else if (c->head_size == 128) launch_types<128>(c->type, a, v.cap, p->n, s);
     else launch_types<256>(c->type, a, v.cap, p->n, s);

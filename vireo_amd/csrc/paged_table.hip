@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(NT) truncate_kernel(TableArgs t, const int32_t
 }
 
 // One workgroup: cut the batch into items. A sequence of u units (kPagedUnit
-// tokens) gets ceil(u / S) items and its units are dealt evenly over them. S is
+// tokens; an empty one has one, of no tokens) gets ceil(u / S) items and its units are dealt evenly over them. S is
 // the batch's units / `whole`, or up to an eighth more, if the items then number
 // at most `whole`: each CU has one, and they end together. Sequences that do not
 // divide so (short ones beside long ones) are cut finer, S = units / `fine`, so that
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__
                                                         int fine, int list_blocks, PlanHead *__restrict__ head,
                                                         PlanSeq *__restrict__ seqs,
                                                         int32_t *__restrict__ first, PlanItem *__restrict__ items,
-                                                        uint32_t tag) {
+                                                        uint32_t *__restrict__ arrivals, int n_arrivals, uint32_t tag) {
     extern __shared__ uint32_t lds[];
     __shared__ uint32_t wsum[2][2][NT / 64], many[3];
     uint32_t *fst = lds, *tok = fst + n + 1;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__
     for (int i = tid; i < n; i += NT) {
         const uint32_t u = (tok[i] + kPagedUnit - 1) / kPagedUnit;
 #pragma unroll
-        for (int k = 0; k < 3; k++) mine[k] += (u + tries[k] - 1) / tries[k];
+        for (int k = 0; k < 3; k++) mine[k] += max((u + tries[k] - 1) / tries[k], 1u);
     }
 #pragma unroll
     for (int k = 0; k < 3; k++)
@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__
         const int i = c + tid;
         uint32_t k = 0;
         if (i < n) {
-            const uint32_t u = (tok[i] + kPagedUnit - 1) / kPagedUnit, m = (u + S - 1) / S;
-            if (m) k = (u + (u + m - 1) / m - 1) / ((u + m - 1) / m);  // items of ceil(u / m) units
+            const uint32_t u = max((tok[i] + kPagedUnit - 1) / kPagedUnit, 1u), m = (u + S - 1) / S;
+            k = (u + (u + m - 1) / m - 1) / ((u + m - 1) / m);  // items of ceil(u / m) units
         }
         uint32_t all;
         const uint32_t f = sum + block_scan<NT>(k, wsum[1][(c / NT) & 1], &all);
@@ -381,8 +381,9 @@ __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__
         const int i = find(fst, n, x);
         const uint32_t k = fst[i + 1] - fst[i], u = (tok[i] + kPagedUnit - 1) / kPagedUnit, per = (u + k - 1) / k;
         const uint32_t b = (x - fst[i]) * per * kPagedUnit, e = min(b + per * kPagedUnit, tok[i]);
-        items[x] = PlanItem{rw[i], int32_t(b), int32_t(e), i | (k == 1 ? int32_t(0x80000000) : 0)};
+        items[x] = PlanItem{rw[i], int32_t(b), int32_t(e), i, int32_t(fst[i]), int32_t(k), {0, 0}};
     }
+    for (int x = tid; x < n_arrivals; x += NT) arrivals[x] = 0;
 }
 
 int log2i(int v) {
@@ -434,7 +435,7 @@ PlanView vh_plan_view(const vireo_paged_plan *p) {
     };
     // no more items than units that the table (or the lists) can hold
     const int64_t most = p->list_blocks && p->list_blocks < p->table->max_blocks ? p->list_blocks : p->table->max_blocks;
-    const int64_t units = (most * p->table->block_tokens + kPagedUnit - 1) / kPagedUnit * p->n;
+    const int64_t each = (most * p->table->block_tokens + kPagedUnit - 1) / kPagedUnit, units = each * p->n;
     v.cap = int(units < plan_slots(p, kFineGroups) + p->n ? units : plan_slots(p, kFineGroups) + p->n);
     v.head = reinterpret_cast<PlanHead *>(take(sizeof(PlanHead)));
     v.seqs = reinterpret_cast<PlanSeq *>(take(int64_t(p->n) * sizeof(PlanSeq)));
@@ -444,6 +445,10 @@ PlanView vh_plan_view(const vireo_paged_plan *p) {
         take(p->list_blocks ? int64_t(p->n) * p->n_kv_heads * p->table->max_blocks * 4 : 0));
     v.ml = reinterpret_cast<float2 *>(take(int64_t(v.cap) * p->n_heads * 8));
     v.part = reinterpret_cast<float *>(take(int64_t(v.cap) * p->n_heads * p->head_size * 4));
+    const int hpg = p->n_heads / p->n_kv_heads;
+    v.join = each <= kJoinUnits && each * (hpg < 16 ? hpg : 16) <= kJoinHeads;
+    if (v.join)
+        v.arrivals = reinterpret_cast<uint32_t *>(take(int64_t(p->n) * p->n_kv_heads * vh_plan_head_tiles(p) * 4));
     v.bytes = at;
     // of the shapes that the memory's layout and its indexes follow from
     uint32_t h = 0x9e3779b9u;
@@ -513,12 +518,15 @@ extern "C" int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream) 
     hipStream_t s = static_cast<hipStream_t>(stream);
     const PlanView v = vh_plan_view(p);
     const size_t lds = 4 * size_t(p->n + 1) + 8 * size_t(p->n);
+    const int n_arrivals = v.join ? p->n * p->n_kv_heads * vh_plan_head_tiles(p) : 0;
     const int whole = plan_slots(p, kWholeGroups), fine = plan_slots(p, kFineGroups);
     if (p->n <= kFewThreads)
         hipLaunchKernelGGL(plan_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), lds, s, args_of(p->table), p->ids, p->n,
-                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
+                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items,
+                           v.arrivals, n_arrivals, v.tag);
     else
         hipLaunchKernelGGL(plan_kernel<kThreads>, dim3(1), dim3(kThreads), lds, s, args_of(p->table), p->ids, p->n,
-                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items, v.tag);
+                           whole, fine, p->list_blocks, v.head, v.seqs, v.first, v.items,
+                           v.arrivals, n_arrivals, v.tag);
     return vh_finish(s, vh_check(hipGetLastError()));
 }

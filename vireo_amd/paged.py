@@ -66,6 +66,7 @@ class _On:
         self.lib = _lib.load()
         self.device = device
         self.index = device.index
+        self.alone = torch.cuda.device_count() == 1
 
     def call(self, name, stream, *args):
         fn = getattr(self.lib, name)
@@ -73,7 +74,7 @@ class _On:
             stream = torch.cuda.current_stream(self.device)
         elif stream.device_index != self.index:
             raise ValueError(f"a stream of {self.device} is needed")
-        if torch.cuda.current_device() == self.index:
+        if self.alone or torch.cuda.current_device() == self.index:
             rc = fn(*args, stream.cuda_stream)
         else:
             with torch.cuda.device(self.device):
