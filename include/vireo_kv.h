@@ -30,6 +30,8 @@
  * result agrees with the reference's sequential online softmax to rounding,
  * and is the same bits whether a block was resident, spilled or paged back.
  *
+ * Many sequences served from one pool in 16 bits: vireo_paged.h.
+ *
  * Vectors (k, v, q, out) are device pointers. Calls enqueue on the given
  * stream (NULL: the null stream, synchronously); every call on a store must use
  * the same stream. A TOPK query copies its block scores to the host and so

@@ -2,7 +2,9 @@
 sizes follow from their shapes. And the plain bookkeeping of the GPU tests, on itself."""
 import ctypes as C
 import errno
+import os
 import random
+import subprocess
 
 import pytest
 
@@ -151,3 +153,15 @@ def test_plain_bookkeeping_keeps_every_block():
             own = [b for r, n in zip(t.blocks, t.len) for b in r[:-(-n // G)]]
             assert sorted(own + t.free[:t.n_free]) == list(range(nb))
     assert seen == {0, EINVAL, E2BIG, ENOSPC}
+
+
+@pytest.mark.parametrize("language", [["-x", "c", "-std=c11"], ["-x", "c++", "-std=c++17"]], ids=["c11", "c++17"])
+def test_header_stands_alone(language):
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    source = """#include <vireo_paged.h>
+int64_t need(const vireo_paged_plan *p);
+int64_t need(const vireo_paged_plan *p) { return vireo_paged_plan_bytes(p); }
+"""
+    r = subprocess.run(["gcc", *language, "-Wall", "-Wextra", "-Wpedantic", "-Werror", "-fsyntax-only", "-I", include, "-"],
+                       input=source, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

@@ -14,9 +14,8 @@
 // transposed while they are reduced (5 exchanges instead of 16). 228 000 mean keys of
 // 128 (58 MB, 16 sequences of 9 000 to 65 536 tokens) against 4 heads each take 19.6 us
 // (24.2 with a block's kv heads far apart in the grid); against one head each 14.2,
-// which is the read; the rest is fp64. The fp64 matrix cores took 46.8 (140 cycles a 16x16x4 product),
-// and 16-bit matrix products that leave only the heads near the highest to fp64 33.9
-// (their operand reads 64 bytes of a key at a time).
+// which is the read; the rest is fp64. The fp64 matrix cores took 46.8, and
+// 16-bit matrix products that leave only the heads near the highest to fp64 33.9.
 // choose_kernel: a workgroup per (sequence, kv head), its keys in registers,
 // finds the budget's lowest score by a histogram of 256 bins of their range and the
 // ranks of the scores in its bin, and writes the blocks in order by one prefix sum.
