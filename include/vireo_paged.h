@@ -123,7 +123,8 @@ typedef struct {
     int rotary;                             /* dimensions rotated, the first ones: a multiple of 16, <= head_size */
     int max_pos;
     const int32_t *positions, *slots;       /* [rows] */
-    void *q_out;                            /* [rows x n_heads x head_size], 16-byte aligned rows; may be q */
+    void *q_out;                            /* [rows x n_heads x head_size], 16-byte aligned rows; may be q, with its
+                                               stride and element size */
     uint32_t q_out_type;                    /* F32 or the cache's */
     int64_t q_out_stride;
 } vireo_paged_rows;
@@ -165,7 +166,7 @@ int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream);
 /* out_i = softmax(scale q_i . K) V over sequence i's tokens, its newest among
  * them (extend and append come first): q, out [n x n_heads x head_size], rows
  * q_stride / out_stride elements apart, of `type` (F32 or the cache's), 16-byte
- * aligned. out may be q. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
+ * aligned. out may be q, with its stride. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
  * are in fp32 or exact: fp32 queries are split into three 16-bit parts, and weights into
  * as many as the output's type needs.
  * lists (NULL unless p->list_blocks > 0): [n x n_kv_heads x list_blocks], for

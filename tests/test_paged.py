@@ -165,3 +165,14 @@ int64_t need(const vireo_paged_plan *p) { return vireo_paged_plan_bytes(p); }
     r = subprocess.run(["gcc", *language, "-Wall", "-Wextra", "-Wpedantic", "-Werror", "-fsyntax-only", "-I", include, "-"],
                        input=source, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.parametrize("kw", [dict(q_out_stride=2048), dict(type=30, q_out_type=0), dict(type=0, q_out_type=30)])
+def test_queries_in_place_keep_their_rows(lib, kw):
+    """q_out at q's address with rows elsewhere or elements of another size would be written over rows still to be read."""
+    assert lib.vireo_paged_append(C.byref(cache()), C.byref(rows(**kw)), None) == BAD
+
+
+def test_attention_in_place_keeps_its_rows(lib):
+    t = table()
+    assert lib.vireo_paged_attend(C.byref(cache()), C.byref(plan(t)), PTR, 30, 1024, 1.0, None, PTR, 2048, None) == BAD

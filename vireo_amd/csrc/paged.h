@@ -38,6 +38,13 @@ inline bool vh_rows_ok(const void *p, uint32_t type, int64_t stride, int64_t hea
     return stride % per16 == 0 && (rows <= 1 || stride >= heads * hs) && stride >= 0 && stride < (int64_t(1) << 40);
 }
 
+// rows written over the ones they are made from have to lie where those lie: others are still to be read
+inline bool vh_in_place_ok(const void *from, uint32_t from_type, int64_t from_stride, const void *to, uint32_t to_type,
+                           int64_t to_stride, int64_t rows) {
+    return from != to || ((from_type == VIREO_PAGED_F32) == (to_type == VIREO_PAGED_F32) &&
+                          (rows <= 1 || from_stride == to_stride));
+}
+
 // ---- a plan's memory ------------------------------------------------------------
 // A batch is cut into items: (sequence, run of kPagedUnit-token units), at least
 // one per sequence. Items of a sequence are consecutive; first[i] is sequence i's

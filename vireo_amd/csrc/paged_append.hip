@@ -211,6 +211,7 @@ extern "C" int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_
         !vh_rows_ok(r->k, r->type, r->k_stride, c->n_kv_heads, hs, r->rows) ||
         !vh_rows_ok(r->v, r->type, r->v_stride, c->n_kv_heads, hs, r->rows) ||
         !vh_rows_ok(r->q_out, r->q_out_type, r->q_out_stride, r->n_heads, hs, r->rows) ||
+        !vh_in_place_ok(r->q, r->type, r->q_stride, r->q_out, r->q_out_type, r->q_out_stride, r->rows) ||
         (r->q_out_type != VIREO_PAGED_F32 && r->q_out_type != c->type) || !r->positions || !r->slots ||
         r->rotary < 0 || r->rotary % 16 || r->rotary > hs || (r->rotary > 0 && (!r->rope || r->max_pos < 1)) ||
         !(r->eps >= 0.0f))

@@ -468,7 +468,8 @@ extern "C" int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_
         c->n_kv_heads != p->n_kv_heads || c->head_size != p->head_size || c->block_tokens != p->table->block_tokens ||
         c->n_blocks != p->table->n_blocks || (type != VIREO_PAGED_F32 && type != c->type) ||
         !vh_rows_ok(q, type, q_stride, p->n_heads, p->head_size, p->n) ||
-        !vh_rows_ok(out, type, out_stride, p->n_heads, p->head_size, p->n) || !(scale > 0.0f && scale < INFINITY) ||
+        !vh_rows_ok(out, type, out_stride, p->n_heads, p->head_size, p->n) ||
+        !vh_in_place_ok(q, type, q_stride, out, type, out_stride, p->n) || !(scale > 0.0f && scale < INFINITY) ||
         (lists != nullptr) != (p->list_blocks > 0))
         return -EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
