@@ -41,9 +41,9 @@
 // Waves merge through LDS. A sequence of one item is then written; others' partial
 // results are joined in the items' order, so that the bits are the same every time:
 // by a second launch (merge_kernel), or, where a sequence can have but few units
-// (short tables and lists of blocks: paged.h), by the last workgroup to arrive. Its inputs are stored and loaded past the dies' L2s (sc1), each store
-// completed before its workgroup counts as arrived: a release fence instead would write back
-// the L2, which costs more than the launch.
+// (short tables and lists of blocks: paged.h), by the last workgroup to arrive. Its
+// inputs are stored and loaded past the dies' L2s (sc1), each store completed before
+// its workgroup counts as arrived: a release fence instead would write back the L2.
 #include <hip/hip_runtime.h>
 #include <errno.h>
 #include "paged.h"

@@ -168,7 +168,7 @@ class PagedPlan:
     def update(self, ids=None, stream=None):
         """By the table's lengths now; ids [n]: the batch's sequences (None: 0 .. n - 1)."""
         self.c.ids = self.table._ids(ids, self.n)
-        self.ids = ids  # select reads it again
+        self.ids = ids  # the update, or a graph that holds it, reads it later
         self.table.on.call("vireo_paged_plan_update", stream, self._p)
 
 
