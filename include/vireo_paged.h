@@ -167,8 +167,7 @@ int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream);
  * them (extend and append come first): q, out [n x n_heads x head_size], rows
  * q_stride / out_stride elements apart, of `type` (F32 or the cache's), 16-byte
  * aligned. out may be q, with its stride. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
- * are in fp32 or exact: fp32 queries are split into three 16-bit parts, and weights into
- * as many as the output's type needs.
+ * are in fp32 or exact: fp32 queries and the weights are split into three 16-bit parts.
  * lists (NULL unless p->list_blocks > 0): [n x n_kv_heads x list_blocks], for
  * each kv head the blocks of the sequence that its heads attend to, by their
  * number in the sequence; only a sequence's first min(its blocks, list_blocks)

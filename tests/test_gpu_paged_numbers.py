@@ -1,0 +1,49 @@
+"""The paged cache's attention at the corners of its arithmetic (include/vireo_paged.h), against fp64 with bounds
+derived from the roundings that are left."""
+import math
+
+import pytest
+import torch
+
+from paged_ref import attend64, half_step
+from test_gpu_paged import BF, F32, HF, Batch, ints, randn
+from vireo_amd import paged as P
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24  # half a step of fp32
+
+
+def working(weight64, size, d):
+    """What fp32 arithmetic before the result's one rounding may be off by (paged_ref.attend_bound without its
+    cut-off weights): 32 + 3 d / 32 half steps of a score into the weights and their sum, 16 for the rest."""
+    return weight64 * (2 * U * ((32 + 3 * d // 32) * size + 16))
+
+
+def check_rounded_once(b, out, scale=None, more=0.0):
+    """Every output is the nearest value of its type to some value within working() of the fp64 result."""
+    scale = 1 / math.sqrt(b.d) if scale is None else scale
+    group = b.H // b.KV
+    for i, t in enumerate(b.lens):
+        for g in range(b.KV):
+            h = slice(g * group, (g + 1) * group)
+            pages = b.rows[b.ids[i]][:-(-t // b.G)]
+            ref, wt, size = attend64(b.q[i, h], b.k[:, g], b.v[:, g], pages,
+                                     [min(b.G, t - x * b.G) for x in range(len(pages))], scale)
+            tol = working(wt, size, b.d) + more
+            # rounding to nearest does not change an order
+            lo, hi = (ref - tol).to(out.dtype), (ref + tol).to(out.dtype)
+            bad = ~((out[i, h] >= lo) & (out[i, h] <= hi))
+            assert not bool(bad.any()), (i, g, t, int(bad.sum()), float((out[i, h].double() - ref).abs().max()))
+
+
+@pytest.mark.parametrize("d,H,KV,G,cache", [(128, 32, 4, 16, BF), (64, 16, 16, 32, BF), (256, 8, 2, 64, BF),
+                                            (128, 32, 4, 16, HF), (256, 8, 2, 16, HF)])
+def test_results_in_16_bits_are_rounded_once(cuda, d, H, KV, G, cache):
+    """Weights in full: values of one sign, a level of its own for every dimension, so that a bias of the weights (of
+    2^-17 of them, if 16 bits were kept) would take results past the borders of their type's values."""
+    lens = [1000, 900, 1, 127, 640, 77, 512, 333]
+    b = Batch(cuda, lens, H, KV, d, G, cache, cache, seed=31, spread=0.02)
+    level = 1 + torch.arange(d, device=cuda) / d
+    live = torch.isfinite(b.v) & (b.v.abs() < 100)  # the junk of unwritten slots stays
+    b.v.copy_(torch.where(live, (level[:, None] + 0.2 * b.v.float()).to(cache), b.v))
+    check_rounded_once(b, b.attend())

@@ -26,15 +26,16 @@
 // 343 -> 318 us, 6.1 TB/s - but for the values of blocks of 64 slots and more, whose lines
 // two tiles share (16 sequences, 275 MB: 78 us with the hint, 67 without; 60 in
 // blocks of 16 and 32). Bound by that read; the matrix cores are busy for 6 % of the
-// time for the 64 sequences (16-bit queries, weights in two parts).
+// time for the 64 sequences (16-bit queries).
 //
 // Precision: products of 16-bit parts are exact in the matrix cores and their
 // sums fp32 (fp16 values below 2^-14 are not flushed, but their products are added
 // as if they were that large: absolute errors of 2^-38 of the largest weight). An fp32
 // query is the sum of three truncated 16-bit parts (fp16: under a power of two per
-// head), and so is a weight for an fp32 result: every bit of them. For a 16-bit
-// result a weight is two parts: 16 bits in bf16, 22 in fp16, with errors under 2^-15
-// and 2^-21 against the result's half step of 2^-8 and 2^-11. The sum of weights is
+// head), and so is a weight, whatever the result's type: a result is rounded once. (Two
+// parts hold 16 bits of a weight in bf16; truncated, they took some results past a
+// border between two bf16 values. The third part's products cost nothing beside the read: 64 sequences 329.4 us with
+// two and 328.4 with three, 131 071 tokens alone 97.2 and 97.4.) The sum of weights is
 // of the fp32 values. Parts that would be zero get the least value of the
 // query's sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
 //
@@ -99,7 +100,7 @@ template <int D, uint32_t T, bool QF, bool ONCE>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArgs a) {
     constexpr int KS = D / 32, DT = D / 16;              // steps of a score, 16-dimension tiles of an output
     constexpr int QP = Queries<D, T, QF>::P;             // parts of a query
-    constexpr int WP = QF ? 3 : 2;                       // parts of a weight
+    constexpr int WP = 3;                                // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
     __shared__ __align__(16) float red[3][16][RS];
     __shared__ float2 wml[4][16];
