@@ -47,3 +47,14 @@ def test_results_in_16_bits_are_rounded_once(cuda, d, H, KV, G, cache):
     live = torch.isfinite(b.v) & (b.v.abs() < 100)  # the junk of unwritten slots stays
     b.v.copy_(torch.where(live, (level[:, None] + 0.2 * b.v.float()).to(cache), b.v))
     check_rounded_once(b, b.attend())
+
+
+@pytest.mark.parametrize("scale,magnitude", [(1e-30, 1e-12), (1 / math.sqrt(128), 4e-41), (1 / math.sqrt(128), 1e-42),
+                                             (1e-45, 1.0), (3e38, 1e-39), (3e38, 1e-44), (1e-38, 1e37), (1e-42, 1e37)])
+def test_scales_and_fp32_queries_of_any_size_over_fp16(cuda, scale, magnitude):
+    """Scale and queries each anywhere in fp32's range, their scores ordinary or as good as 0 (then every weight is the
+    same); lengths that fill their last tile and lengths that do not."""
+    b = Batch(cuda, [300, 65, 1000, 31, 128], 8, 2, 128, 16, HF, F32, seed=33)
+    b.q *= magnitude
+    scale = float(torch.tensor(scale, dtype=F32))
+    b.check(b.attend(scale=scale), scale=scale)

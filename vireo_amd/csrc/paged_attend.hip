@@ -47,12 +47,12 @@
 // its workgroup counts as arrived: a release fence instead would write back the L2.
 #include <hip/hip_runtime.h>
 #include <errno.h>
+#include <math.h>
 #include "paged.h"
 
 namespace {
 
 constexpr float kLowest = -3.4028234663852886e38f;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
     const uint16_t *k, *v;
@@ -63,7 +63,8 @@ struct AttendArgs {
     int list_blocks;
     const void *q;
     int64_t q_stride;
-    float c;  // scale log2(e): scores in powers of two
+    float mant;  // scale log2(e) = mant 2^expo: scores in powers of two
+    int expo;
     int n_heads, hpg, tiles;  // query heads, of a kv head, tiles of 16 of those
     void *out;
     int64_t out_stride;
@@ -203,7 +204,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     __builtin_amdgcn_sched_barrier(0);
     u32x4 qw[QP][KS];
     const int e = query.parts(qw);
-    const float c = ldexpf(ldexpf(a.c, -(e / 2)), e / 2 - e);  // in two steps: 2^e alone may leave fp32's range
+    // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
+    // scale 2^-e lies under 2^-126: all weights are 1 either way.
+    const float c = ldexpf(a.mant, min(max(a.expo - e, -126), 126));
     if (i0 < i1) {
         for (int i = i0; i < i1; i++) {
             f32x4 s[2];
@@ -477,9 +480,11 @@ extern "C" int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_
     const PlanView v = vh_plan_view(p);
     int shift = 4;
     while ((1 << shift) < c->block_tokens) shift++;
+    int expo;
+    const double mant = 2.0 * frexp(double(scale) * 1.4426950408889634, &expo);
     const AttendArgs a{static_cast<const uint16_t *>(c->k), static_cast<const uint16_t *>(c->v), c->n_blocks,
                        c->n_kv_heads, shift, p->table->blocks, p->table->len, p->table->max_blocks, lists,
-                       p->list_blocks, q, q_stride, scale * kLog2e, p->n_heads, p->n_heads / p->n_kv_heads,
+                       p->list_blocks, q, q_stride, float(mant), expo - 1, p->n_heads, p->n_heads / p->n_kv_heads,
                        vh_plan_head_tiles(p), out, out_stride, type, v.head, v.items, v.first, v.tag, v.part, v.ml, v.arrivals};
     if (c->head_size == 64) launch_types<64>(c->type, a, v.cap, p->n, s);
     else if (c->head_size == 128) launch_types<128>(c->type, a, v.cap, p->n, s);
