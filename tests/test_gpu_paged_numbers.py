@@ -58,3 +58,28 @@ def test_scales_and_fp32_queries_of_any_size_over_fp16(cuda, scale, magnitude):
     b.q *= magnitude
     scale = float(torch.tensor(scale, dtype=F32))
     b.check(b.attend(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("cache,query,big,step", [(BF, BF, 2.0 ** 40, 1.0), (BF, BF, 2.0 ** 100, 1.0), (BF, F32, 1.7e30, 1.0),
+                                                  (HF, HF, 60000.0, 1024.0), (HF, F32, 1.7e10, 1.0), (HF, F32, 3e33, 16.0)])
+def test_scores_of_any_size(cuda, cache, query, big, step):
+    """Scores so large that only the largest has a weight: queries of one dimension and keys of few bits there, so that
+    every sum is exact and the largest, at two tokens of each sequence, far above the next. The result is the mean of their
+    values (weights of 1 and 0)."""
+    b = Batch(cuda, [300, 65, 3000, 31, 128], 8, 2, 128, 16, cache, query, seed=34)
+    b.q.zero_()
+    b.q[:, :, 5] = big
+    live = torch.isfinite(b.k) & (b.k.abs() < 100)
+    b.k.copy_(torch.where(live, torch.round(b.k * 4) * step, b.k))
+    tops = [(t // 3, t - 2) for t in b.lens]
+    for i, ts in enumerate(tops):
+        for t in ts:
+            b.k[b.rows[b.ids[i]][t // 16], :, t % 16, 5] = 27 * step
+    out = b.attend()
+    for i, ts in enumerate(tops):
+        at = [(b.rows[b.ids[i]][t // 16], t % 16) for t in ts]
+        for g in range(2):
+            vv = torch.stack([b.v[p, g, :, o] for p, o in at]).double()
+            want, tol = vv.mean(0), working(vv.abs().mean(0), 0.0, 128)
+            err = (out[i, 4 * g:4 * g + 4].double() - want).abs()
+            assert bool((err <= half_step(query) * want.abs() + tol).all()), (i, g, float(err.max()))

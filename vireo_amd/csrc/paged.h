@@ -77,7 +77,7 @@ struct PlanView {
     int32_t *first;   // [n + 1]
     PlanItem *items;  // [cap]
     uint32_t *keys;   // [n x n_kv_heads x max_blocks] ordered scores (plans with lists)
-    float2 *ml;       // [cap x n_heads] largest score and sum of weights of each item's partial
+    float2 *ml;       // [cap x n_heads] largest score (times a power of two) and sum of weights of each item's partial
     float *part;      // [cap x n_heads x head_size]
     uint32_t *arrivals;  // [n x n_kv_heads x head tiles], zero between calls
     int cap;

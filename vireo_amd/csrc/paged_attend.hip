@@ -13,7 +13,7 @@
 //                 results of a lane from each are its head's scores of tokens
 //                 8 g .. 8 g + 7 (g = lane / 16).
 //   weights       an online softmax: the running maximum over the head's four
-//                 lanes, e^(s - m) in fp32, the sum per lane.
+//                 lanes, e^(scale (s - m)) in fp32, the sum per lane.
 //   O^T += V^T P^T  rows are 16 dimensions, columns the heads, the 32 the tile's
 //                 tokens: the lane's 8 weights are its operand as they stand, and 16
 //                 consecutive bytes of the cache (8 tokens of a dimension) are V^T's.
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     const int e = query.parts(qw);
     // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
     // scale 2^-e lies under 2^-126: all weights are 1 either way.
-    const float c = ldexpf(a.mant, min(max(a.expo - e, -126), 126));
+    const float two = ldexpf(1.0f, min(max(a.expo - e, -126), 126)), c = a.mant * two;
     if (i0 < i1) {
         for (int i = i0; i < i1; i++) {
             f32x4 s[2];
@@ -246,15 +246,15 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             float mx = x[0];
 #pragma unroll
             for (int j = 1; j < 8; j++) mx = fmaxf(mx, x[j]);
-            const float mn = fmaxf(m, head_max(mx) * c);
-            const float cr = __builtin_amdgcn_exp2f(m - mn);
+            const float mn = fmaxf(m, head_max(mx));
+            const float cr = __builtin_amdgcn_exp2f((m - mn) * c);
             m = mn;
-            // fp16's parts: weights up to 2^14, so that small ones keep their bits
-            const float up = T == VIREO_PAGED_F16 ? 14.0f - m : -m;
             float ps = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, up));
+                // the difference before the scale: that of a large score's rounding would be an exponent. fp16's
+                // parts: weights up to 2^14, so that small ones keep their bits
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j] - m, c, T == VIREO_PAGED_F16 ? 14.0f : 0.0f));
                 ps += x[j];
             }
             l = fmaf(l, cr, ps);
@@ -272,8 +272,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     }
     l = head_sum(l);
     if (T == VIREO_PAGED_F16) l = l * 0x1p-14f;
-    // the waves' maxima; -inf marks a wave that attended nothing
-    if (grp == 0) wml[wv][col] = make_float2(seen ? m : -INFINITY, l);
+    // the waves' maxima, from here on in units of the scale's mantissa (exact, so that those of equal scores stay
+    // equal); -inf marks a wave that attended nothing
+    if (grp == 0) wml[wv][col] = make_float2(seen ? fmaxf(m * two, kLowest) : -INFINITY, l);
     __syncthreads();
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float2 o = wml[w][col];
-            const float fw = __builtin_amdgcn_exp2f(o.x - M);
+            const float fw = __builtin_amdgcn_exp2f((o.x - M) * a.mant);
             L = fmaf(o.y, fw, L);
             f = w == wv ? fw : f;
         }
@@ -366,13 +367,13 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
 #pragma unroll
                 for (int u = 0; u < U; u++) big = fmaxf(big, __uint_as_float(ml[x][u][0]));  // repeats of the last one too
                 if (big == -INFINITY) continue;
-                const float back = __builtin_amdgcn_exp2f(m1[x] - big);
+                const float back = __builtin_amdgcn_exp2f((m1[x] - big) * a.mant);
                 l1[x] *= back;
                 y[x] *= back;
 #pragma unroll
                 for (int u = 0; u < U; u++)
                     if (i0 + u < it.count) {
-                        const float f1 = __builtin_amdgcn_exp2f(__uint_as_float(ml[x][u][0]) - big);
+                        const float f1 = __builtin_amdgcn_exp2f((__uint_as_float(ml[x][u][0]) - big) * a.mant);
                         l1[x] = fmaf(__uint_as_float(ml[x][u][1]), f1, l1[x]);
                         y[x] += __builtin_bit_cast(f32x4, v[x][u]) * f1;
                     }
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
         float f = 0.0f, l = 0.0f;
         if (tid < m) {
             const float2 o = ml[size_t(i0 + tid) * a.n_heads];
-            if (o.x > -INFINITY) f = __builtin_amdgcn_exp2f(o.x - M), l = o.y * f;
+            if (o.x > -INFINITY) f = __builtin_amdgcn_exp2f((o.x - M) * a.mant), l = o.y * f;
         }
         fs[tid] = f;
         l = wave_sum_f(l);
