@@ -83,3 +83,66 @@ def test_scores_of_any_size(cuda, cache, query, big, step):
             want, tol = vv.mean(0), working(vv.abs().mean(0), 0.0, 128)
             err = (out[i, 4 * g:4 * g + 4].double() - want).abs()
             assert bool((err <= half_step(query) * want.abs() + tol).all()), (i, g, float(err.max()))
+
+
+@pytest.mark.parametrize("query", [HF, F32])
+def test_tokens_without_weight_add_nothing(cuda, query):
+    """One token's weight is e^44 times every other's, whose values are 60 000 times its own: 32 767 of them add
+    10^-10 to a result of 1. 256 sequences that are the same, so that each is one workgroup's and the others follow the one
+    in its wave."""
+    G, n, t, d = 16, 256, 32768, 64
+    k, v = torch.zeros((t // G, 1, G, d), dtype=HF, device=cuda), torch.full((t // G, 1, d, G), 60000.0, dtype=HF, device=cuda)
+    k[0, 0, 0, 0], v[0, 0, :, 0] = 44.0, 1.0
+    table = P.PagedTable(torch.arange(t // G, dtype=torch.int32, device=cuda)[None].contiguous(), ints([t], cuda),
+                         torch.zeros(t // G, dtype=torch.int32, device=cuda), ints([0], cuda), G)
+    cache = P.PagedCache(k, v)
+    plan = P.PagedPlan(table, cache, n, 1)
+    plan.update(ids=torch.zeros(n, dtype=torch.int32, device=cuda))
+    q = torch.zeros((n, 1, d), dtype=query, device=cuda)
+    q[:, :, 0] = 1.0
+    out = torch.empty_like(q)
+    cache.attend(q, out, plan, scale=1.0)
+    want = 1 + 32767 * math.exp(-44) * 60000
+    err = (out.double() - want).abs().max()
+    assert float(err) <= half_step(query) + float(working(torch.tensor(1.0), 44.0, d)), float(err)
+
+
+@pytest.mark.parametrize("query", [BF, F32])
+def test_large_values_under_a_weight_of_zero(cuda, query):
+    """Values of 3 10^38 where the key makes a score of -inf add nothing."""
+    b = Batch(cuda, [40, 200], 4, 2, 64, 16, BF, query, seed=35)
+    b.q[:, :, 0] = b.q[:, :, 0].abs() + 0.5
+    clean = [b.k.clone(), b.v.clone()]
+    for i, first in ((0, 3), (1, 150)):
+        for x in range(first, b.lens[i]):
+            p, o = b.rows[b.ids[i]][x // 16], x % 16
+            b.k[p, :, o, 0], b.v[p, :, :, o] = -math.inf, 3e38
+    out = b.attend()
+    b.k, b.v, b.lens = *clean, [3, 150]
+    b.check(out)
+
+
+@pytest.mark.parametrize("cache,query", [(BF, BF), (BF, F32), (HF, HF), (HF, F32)])
+@pytest.mark.parametrize("gap,d,G", [(0.0, 64, 16), (5.0, 128, 64), (20.0, 256, 16), (44.0, 64, 128), (44.0, 128, 16),
+                                     (80.0, 64, 16), (80.0, 256, 64)])
+def test_infinite_values_under_any_weight(cuda, cache, query, gap, d, G):
+    """A token's infinite value makes its dimension infinite under every weight that fp32 holds, e^-80 of the largest
+    too, in tiles before and after the largest; one of each sign, or a NaN, makes it a NaN; other dimensions keep their bits."""
+    b = Batch(cuda, [200, 2000, 33], 4, 2, d, G, cache, query, seed=36)
+    live = torch.isfinite(b.k) & (b.k.abs() < 100)
+    b.k.copy_(torch.where(live, torch.zeros_like(b.k), b.k))
+    b.q.fill_(1.0)
+    spots = [[3, 150, 77], [40, 1990, 1033], [2, 32, 17]]
+    for i, ts in enumerate(spots):
+        for t in ts:
+            b.k[b.rows[b.ids[i]][t // G], :, t % G, 1] = -gap
+    clean = b.attend(scale=1.0)
+    b.check(clean, scale=1.0)
+    want = clean.clone()
+    for i, ts in enumerate(spots):
+        for t, dim, value in zip(ts + ts, (5, 6, 7, 8, 8, 9), (math.inf, -math.inf, math.nan, math.inf, -math.inf, -math.inf)):
+            b.v[b.rows[b.ids[i]][t // G], 1, dim, t % G] = value
+        want[i, 2:, 5], want[i, 2:, 6], want[i, 2:, 9] = math.inf, -math.inf, -math.inf
+        want[i, 2:, 7] = want[i, 2:, 8] = math.nan
+    out = b.attend(scale=1.0)
+    assert bool(((out == want) | (torch.isnan(out) & torch.isnan(want))).all())

@@ -180,9 +180,9 @@ VH_DEV float head_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// x split into NP truncated 16-bit parts, the operand words of each; x >= 0
-// elements stay >= 0. Zero parts of a nonzero x become the least value.
-template <uint32_t T, int NP>
+// x split into NP truncated 16-bit parts, the operand words of each. LEAST: zero parts
+// but the first become the least value of x's sign.
+template <uint32_t T, int NP, bool LEAST>
 VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
@@ -190,7 +190,7 @@ VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             if constexpr (T == VIREO_PAGED_BF16) {
-                if (p) {  // 2^-126, of the value's sign
+                if (LEAST && p) {  // 2^-126
                     a = copysignf(fmaxf(fabsf(a), 1.17549435e-38f), x[j]);
                     b = copysignf(fmaxf(fabsf(b), 1.17549435e-38f), x[j + 1]);
                 }
@@ -199,7 +199,7 @@ VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
                 a -= __uint_as_float(ua & 0xffff0000u);
                 b -= __uint_as_float(ub & 0xffff0000u);
             } else {
-                if (p) {  // 2^-24
+                if (LEAST && p) {  // 2^-24
                     a = copysignf(fmaxf(fabsf(a), 5.9604645e-8f), x[j]);
                     b = copysignf(fmaxf(fabsf(b), 5.9604645e-8f), x[j + 1]);
                 }
@@ -258,7 +258,7 @@ struct Queries {
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 u32x4 p[3];
-                split8<T, 3>(x[s], p);
+                split8<T, 3, true>(x[s], p);
 #pragma unroll
                 for (int k = 0; k < 3; k++) w[k][s] = p[k];
             }

@@ -36,8 +36,12 @@
 // parts hold 16 bits of a weight in bf16; truncated, they took some results past a
 // border between two bf16 values. The third part's products cost nothing beside the read: 64 sequences 329.4 us with
 // two and 328.4 with three, 131 071 tokens alone 97.2 and 97.4.) The sum of weights is
-// of the fp32 values. Parts that would be zero get the least value of the
+// of the fp32 values. Over fp16 a weight is cut off at 2^-38 of the largest that its
+// wave has seen. Parts of a query that would be zero get the least value of the
 // query's sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
+// A weight's are left: that much from each of many tokens without weight would be seen
+// beside a few that have it. A NaN that an infinite value may have made so is put right
+// at the end.
 //
 // Waves merge through LDS. A sequence of one item is then written; others' partial
 // results are joined in the items' order, so that the bits are the same every time:
@@ -103,7 +107,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     constexpr int QP = Queries<D, T, QF>::P;             // parts of a query
     constexpr int WP = 3;                                // parts of a weight
     constexpr int RS = D + 4;                            // LDS row of a head: its 16 lanes on different banks
-    __shared__ __align__(16) float red[3][16][RS];
+    __shared__ __align__(16) float red[4][16][RS];
     __shared__ float2 wml[4][16];
     // heads vary fastest: a block's kv heads are neighbours in memory, and the
     // plan's unused items come last
@@ -207,17 +211,40 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
     // scale 2^-e lies under 2^-126: all weights are 1 either way.
     const float two = ldexpf(1.0f, min(max(a.expo - e, -126), 126)), c = a.mant * two;
+    // the lane's 8 scores of the tile in kk
+    auto scores = [&](float (&x)[8]) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = QP - 1; p >= 0; p--)
+#pragma unroll
+                for (int k = 0; k < KS; k++) s = El<T>::mfma(kk[u][k], qw[p][k], s);
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[4 * u + j] = s[j];
+        }
+    };
+    // no score and no value for slots that are not attended: what lies there is not to meet a weight of 0, it may be
+    // an infinity or a NaN
+    auto mask = [&](const Where &w, float (&x)[8]) {
+        if (w.n[0] == 16 && w.n[1] == 16) return;  // the same on every lane
+        // slots of the lane's 8 that are attended
+        const int nv = min(max((grp >> 1 ? w.n[1] : w.n[0]) - 8 * (grp & 1), 0), 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = j < nv ? x[j] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t keep = nv >= 2 * j + 2 ? 0xffffffffu : nv == 2 * j + 1 ? 0xffffu : 0u;
+#pragma unroll
+            for (int d = 0; d < DT; d++) vv[d][j] &= keep;
+        }
+    };
+    // a weight, at most 1 (the difference before the scale: a large score's rounding would be an exponent); over fp16 up to 2^14, so that the parts of small ones keep their bits
+    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x - m, c, T == VIREO_PAGED_F16 ? 14.0f : 0.0f)); };
     if (i0 < i1) {
         for (int i = i0; i < i1; i++) {
-            f32x4 s[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int p = QP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int k = 0; k < KS; k++) s[u] = El<T>::mfma(kk[u][k], qw[p][k], s[u]);
-            }
+            float x[8];
+            scores(x);
             const bool more = i + 1 < i1;
             Where next = w;
             if (more) {
@@ -225,24 +252,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
                 next = where(i + 1);
                 load_k(next);
             }
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3];
-            const bool whole = w.n[0] == 16 && w.n[1] == 16;  // the same on every lane
-            // slots of the lane's 8 that are attended
-            const int nv = whole ? 8 : min(max((grp >> 1 ? w.n[1] : w.n[0]) - 8 * (grp & 1), 0), 8);
             seen |= w.n[0] + w.n[1] > 0;
-            if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = j < nv ? x[j] : -INFINITY;
-                // what lies in the other slots is not to meet a weight of 0: it may be an infinity or a NaN
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t keep = nv >= 2 * j + 2 ? 0xffffffffu : nv == 2 * j + 1 ? 0xffffu : 0u;
-#pragma unroll
-                    for (int d = 0; d < DT; d++) vv[d][j] &= keep;
-                }
-            }
+            mask(w, x);
             float mx = x[0];
 #pragma unroll
             for (int j = 1; j < 8; j++) mx = fmaxf(mx, x[j]);
@@ -252,14 +263,12 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             float ps = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                // the difference before the scale: that of a large score's rounding would be an exponent. fp16's
-                // parts: weights up to 2^14, so that small ones keep their bits
-                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j] - m, c, T == VIREO_PAGED_F16 ? 14.0f : 0.0f));
+                x[j] = weight(x[j]);
                 ps += x[j];
             }
             l = fmaf(l, cr, ps);
             u32x4 pw[WP];
-            split8<T, WP>(x, pw);
+            split8<T, WP, false>(x, pw);
 #pragma unroll
             for (int d = 0; d < DT; d++) acc[d] *= cr;
 #pragma unroll
@@ -268,6 +277,48 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
                 for (int p = WP - 1; p >= 0; p--) acc[d] = El<T>::mfma(vv[d], pw[p], acc[d]);
             w = next;
             if (more) load_v(w);
+        }
+    }
+    // A NaN may be an infinite value's, under a weight of which a part is 0: what such values (and NaN) come to under
+    // weights of 1 and 0 takes its place. Rare, and looked for once: 8 to 32 comparisons a wave.
+    bool odd = false;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+        odd |= __builtin_isunordered(acc[d][0], acc[d][1]) || __builtin_isunordered(acc[d][2], acc[d][3]);
+    if (__any(odd)) {
+        // the results so far are put aside: they would take registers that the loop above could not have
+        float *aside = &red[wv][col][4 * grp];
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            *reinterpret_cast<f32x4 *>(aside + 16 * d) = acc[d];
+            acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        blocks_from((it.begin + 32 * i0) >> shift);
+        for (int i = i0; i < i1; i++) {
+            if (((it.begin + 32 * i + 31) >> shift) - e0 >= 64) blocks_from((it.begin + 32 * i) >> shift);
+            w = where(i);
+            load_k(w);
+            float x[8];
+            scores(x);
+            __builtin_amdgcn_sched_barrier(0);  // values into the keys' registers: no more of them than in the loop above
+            load_v(w);
+            mask(w, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[j] = weight(x[j]);
+                x[j] = x[j] > 0.0f ? 1.0f : x[j];  // a NaN stays one
+            }
+            u32x4 pw;
+#pragma unroll
+            for (int j = 0; j < 4; j++) pw[j] = El<T>::pack(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] = El<T>::mfma(vv[d], pw, acc[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(aside + 16 * d);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[d][j] = y[j] != y[j] && !(fabsf(acc[d][j]) < INFINITY) ? acc[d][j] : y[j];
         }
     }
     l = head_sum(l);
