@@ -146,3 +146,39 @@ def test_infinite_values_under_any_weight(cuda, cache, query, gap, d, G):
         want[i, 2:, 7] = want[i, 2:, 8] = math.nan
     out = b.attend(scale=1.0)
     assert bool(((out == want) | (torch.isnan(out) & torch.isnan(want))).all())
+
+
+@pytest.mark.parametrize("cache", [BF, HF])
+def test_zero_elements_of_fp32_queries(cuda, cache):
+    """Where a query's element is 0 the key's does not count, however large: the scores are 0, the weights equal."""
+    b = Batch(cuda, [300, 65, 1000], 8, 2, 128, 16, cache, F32, seed=37)
+    live = torch.isfinite(b.k) & (b.k.abs() < 100)
+    large = torch.where(b.k > 0, 6e4, -6e4) if cache is HF else torch.where(b.k > 0, 3e38, -3e38)
+    large[..., 0] = 0.0
+    b.k.copy_(torch.where(live, large.to(cache), b.k))
+    b.q.zero_()
+    b.q[:, :, 0] = 1e4
+    b.check(b.attend())
+
+
+@pytest.mark.parametrize("magnitude,scale", [(1e-30, 1e30), (1e-35, 1e35), (1e-37, 1e37), (1e-38, 1e38), (1e-41, 3e38), (1e30, 1e-30)])
+def test_fp32_queries_of_any_size_over_bf16(cuda, magnitude, scale):
+    """Parts of a small query are not lost below bf16's least normal value (2^-126)."""
+    b = Batch(cuda, [300, 65, 1000], 8, 2, 128, 16, BF, F32, seed=38)
+    b.q *= magnitude
+    scale = float(torch.tensor(scale / math.sqrt(128), dtype=F32))
+    b.check(b.attend(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("cache,small", [(BF, 1e-30), (BF, 1e-40), (HF, 1e-4), (HF, 1e-20), (HF, 1e-40)])
+def test_infinite_keys_of_any_element(cuda, cache, small):
+    """A key of -inf makes a score of -inf with a query's element however small, its largest being about 1."""
+    b = Batch(cuda, [100, 400], 8, 2, 64, 16, cache, F32, seed=39)
+    b.q[:, :, 9] = small
+    clean = [b.k.clone(), b.v.clone()]
+    for i, first in ((0, 60), (1, 300)):
+        for x in range(first, b.lens[i]):
+            b.k[b.rows[b.ids[i]][x // 16], :, x % 16, 9] = -math.inf
+    out = b.attend()
+    b.k, b.v, b.lens = *clean, [60, 300]
+    b.check(out)

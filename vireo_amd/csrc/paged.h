@@ -180,29 +180,32 @@ VH_DEV float head_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// x split into NP truncated 16-bit parts, the operand words of each. LEAST: zero parts
-// but the first become the least value of x's sign.
+// x split into NP truncated 16-bit parts, the operand words of each. LEAST: parts of an x
+// that is not 0 which would be 0 become the least value of its sign.
 template <uint32_t T, int NP, bool LEAST>
 VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
+    constexpr float kLeast = T == VIREO_PAGED_BF16 ? 1.17549435e-38f : 5.9604645e-8f;  // 2^-126, 2^-24
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-        float a = x[j], b = x[j + 1];
+        float a = x[j], b = x[j + 1], la = 0.0f, lb = 0.0f;
+        if constexpr (LEAST) {
+            la = fminf(fabsf(a) * 0x1p127f, kLeast);  // 0 for a zero
+            lb = fminf(fabsf(b) * 0x1p127f, kLeast);
+            a = fabsf(a) < la ? copysignf(la, a) : a;
+            b = fabsf(b) < lb ? copysignf(lb, b) : b;
+        }
 #pragma unroll
         for (int p = 0; p < NP; p++) {
+            if (LEAST && p) {
+                a = copysignf(fmaxf(fabsf(a), la), x[j]);
+                b = copysignf(fmaxf(fabsf(b), lb), x[j + 1]);
+            }
             if constexpr (T == VIREO_PAGED_BF16) {
-                if (LEAST && p) {  // 2^-126
-                    a = copysignf(fmaxf(fabsf(a), 1.17549435e-38f), x[j]);
-                    b = copysignf(fmaxf(fabsf(b), 1.17549435e-38f), x[j + 1]);
-                }
                 const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
                 w[p][j / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);  // the high halves
                 a -= __uint_as_float(ua & 0xffff0000u);
                 b -= __uint_as_float(ub & 0xffff0000u);
             } else {
-                if (LEAST && p) {  // 2^-24
-                    a = copysignf(fmaxf(fabsf(a), 5.9604645e-8f), x[j]);
-                    b = copysignf(fmaxf(fabsf(b), 5.9604645e-8f), x[j + 1]);
-                }
                 const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
                 w[p][j / 2] = __builtin_bit_cast(uint32_t, h);
                 a -= float(h[0]);
@@ -214,9 +217,11 @@ VH_DEV void split8(const float (&x)[8], u32x4 (&w)[NP]) {
 
 // A matrix operand of queries of type F32 (QF) or T as parts of T: lane (col,
 // grp) loads values 32 s + 0 .. 7 from element `at` on (its head's, 8 grp in) for
-// each step s; load() only requests them, parts() waits. fp32 queries over fp16 are
-// taken under a power of two that brings the head's largest into [2^14, 2^15);
-// parts() returns its exponent.
+// each step s; load() only requests them, parts() waits. fp32 queries are taken under a
+// power of two whose exponent parts() returns: over fp16 one that brings the head's largest
+// into [2^14, 2^15), so that a value is cut off at 2^-38 of it; over bf16 one that
+// brings it to 2^-60 where it is smaller, for the parts' sake (larger ones could
+// leave fp32 with the keys). LEAST: as split8's.
 template <int D, uint32_t T, bool QF>
 struct Queries {
     static constexpr int KS = D / 32, P = QF ? 3 : 1;
@@ -233,6 +238,7 @@ struct Queries {
             }
         }
     }
+    template <bool LEAST>
     VH_DEV int parts(u32x4 (&w)[P][KS]) const {
         int e = 0;
         if constexpr (!QF) {
@@ -247,9 +253,10 @@ struct Queries {
                     x[s][j] = __uint_as_float(raw[s][j >> 2][j & 3]);
                     big = fmaxf(big, fabsf(x[s][j]));
                 }
-            if constexpr (T == VIREO_PAGED_F16) {
+            if (T == VIREO_PAGED_F16 || __any(big < 0x1p-60f)) {
                 big = head_max(big);
-                if (big > 0.0f && big < INFINITY) e = 14 - ilogbf(big);
+                if (T == VIREO_PAGED_F16 ? big > 0.0f && big < INFINITY : big > 0.0f && big < 0x1p-60f)
+                    e = (T == VIREO_PAGED_F16 ? 14 : -60) - ilogbf(big);
 #pragma unroll
                 for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -258,7 +265,7 @@ struct Queries {
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 u32x4 p[3];
-                split8<T, 3, true>(x[s], p);
+                split8<T, 3, LEAST>(x[s], p);
 #pragma unroll
                 for (int k = 0; k < 3; k++) w[k][s] = p[k];
             }

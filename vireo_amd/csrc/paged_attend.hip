@@ -31,17 +31,16 @@
 // Precision: products of 16-bit parts are exact in the matrix cores and their
 // sums fp32 (fp16 values below 2^-14 are not flushed, but their products are added
 // as if they were that large: absolute errors of 2^-38 of the largest weight). An fp32
-// query is the sum of three truncated 16-bit parts (fp16: under a power of two per
-// head), and so is a weight, whatever the result's type: a result is rounded once. (Two
+// query is the sum of three truncated 16-bit parts (under a power of two per
+// head: Queries), and so is a weight, whatever the result's type: a result is rounded once. (Two
 // parts hold 16 bits of a weight in bf16; truncated, they took some results past a
 // border between two bf16 values. The third part's products cost nothing beside the read: 64 sequences 329.4 us with
 // two and 328.4 with three, 131 071 tokens alone 97.2 and 97.4.) The sum of weights is
-// of the fp32 values. Over fp16 a weight is cut off at 2^-38 of the largest that its
-// wave has seen. Parts of a query that would be zero get the least value of the
-// query's sign, so that an infinite key gives an infinite score and not 0 inf = NaN.
-// A weight's are left: that much from each of many tokens without weight would be seen
-// beside a few that have it. A NaN that an infinite value may have made so is put right
-// at the end.
+// of the fp32 values. Over fp16 a query's value is cut off at 2^-38 of the head's
+// largest, a weight at 2^-38 of the largest that its wave has seen. Infinite keys and
+// values meet parts that are 0, whose products are NaN: where a wave finds a NaN in its sums it
+// goes over its tiles again, with the least value of its sign in place of such parts of a query's
+// value (in every call that would be seen beside large keys), and with weights of 1 and 0.
 //
 // Waves merge through LDS. A sequence of one item is then written; others' partial
 // results are joined in the items' order, so that the bits are the same every time:
@@ -125,7 +124,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
     // the queries: column col's head, dimensions 32 s + 8 grp .. + 7 of step s
     // (formed below, once the first keys and values are requested too)
     Queries<D, T, QF> query;
-    query.load(a.q, seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp);
+    const int64_t q0 = seq * a.q_stride + int64_t(h0 + min(col, nh - 1)) * D + 8 * grp;
+    query.load(a.q, q0);
 
     // the wave's tiles, and the blocks behind them, 64 at a time: lane e holds
     // block e0 + e of the sequence (or of its list) and how many of its slots
@@ -196,21 +196,12 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
         }
     };
 
-    float m = kLowest, l = 0.0f;
+    float m, l;
     bool seen = false;  // a token was attended
     f32x4 acc[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    blocks_from((it.begin + 32 * i0) >> shift);
-    Where w = where(i0);  // i0 < T0; a wave without tiles reads one that it does not use
-    load_k(w);
-    load_v(w);
-    __builtin_amdgcn_sched_barrier(0);
+    Where w;
     u32x4 qw[QP][KS];
-    const int e = query.parts(qw);
-    // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
-    // scale 2^-e lies under 2^-126: all weights are 1 either way.
-    const float two = ldexpf(1.0f, min(max(a.expo - e, -126), 126)), c = a.mant * two;
+    float two, c;
     // the lane's 8 scores of the tile in kk
     auto scores = [&](float (&x)[8]) {
 #pragma unroll
@@ -239,9 +230,28 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             for (int d = 0; d < DT; d++) vv[d][j] &= keep;
         }
     };
-    // a weight, at most 1 (the difference before the scale: a large score's rounding would be an exponent); over fp16 up to 2^14, so that the parts of small ones keep their bits
+    // a weight, at most 1 (the difference before the scale: a large score's rounding would be an exponent); over fp16
+    // up to 2^14, so that the parts of small ones keep their bits
     auto weight = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x - m, c, T == VIREO_PAGED_F16 ? 14.0f : 0.0f)); };
-    if (i0 < i1) {
+    for (bool again = false;; again = true) {
+        m = kLowest, l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        blocks_from((it.begin + 32 * i0) >> shift);
+        w = where(i0);  // i0 < T0 but where T0 = 0; a wave without tiles reads one that it does not use
+        load_k(w);
+        load_v(w);
+        __builtin_amdgcn_sched_barrier(0);
+        int e;
+        if (QF && again) {
+            query.load(a.q, q0);
+            e = query.template parts<true>(qw);
+        } else {
+            e = query.template parts<false>(qw);
+        }
+        // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
+        // scale 2^-e lies under 2^-126: all weights are 1 either way.
+        two = ldexpf(1.0f, min(max(a.expo - e, -126), 126)), c = a.mant * two;
         for (int i = i0; i < i1; i++) {
             float x[8];
             scores(x);
@@ -278,6 +288,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             w = next;
             if (more) load_v(w);
         }
+        // A NaN may be an infinite key's, with a part of a query's value that is 0: once more, without such parts.
+        if (!QF || again || !__any(l != l)) break;
     }
     // A NaN may be an infinite value's, under a weight of which a part is 0: what such values (and NaN) come to under
     // weights of 1 and 0 takes its place. Rare, and looked for once: 8 to 32 comparisons a wave.
