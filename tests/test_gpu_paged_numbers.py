@@ -182,3 +182,19 @@ def test_infinite_keys_of_any_element(cuda, cache, small):
     out = b.attend()
     b.k, b.v, b.lens = *clean, [60, 300]
     b.check(out)
+
+
+# ---- the largest sizes ----------------------------------------------------------------------------------------------
+
+def test_plan_of_more_units_than_a_sum_holds(cuda):
+    """4 096 times one sequence of 2^31 - 32 tokens: 2^36 units of 128, past the 31 bits of the plan's sums. No more
+    items than the plan's memory holds (2 048 and one more per sequence), and each sequence has one."""
+    G, n = 16, 4096
+    width = 2 ** 27 - 2
+    table = P.PagedTable(torch.zeros((1, width), dtype=torch.int32, device=cuda), ints([width * G], cuda),
+                         torch.zeros(8, dtype=torch.int32, device=cuda), ints([0], cuda), G)
+    cache = P.PagedCache(*(torch.zeros(s, dtype=BF, device=cuda) for s in ((8, 1, G, 64), (8, 1, 64, G))))
+    plan = P.PagedPlan(table, cache, n, 1)
+    plan.update(ids=torch.zeros(n, dtype=torch.int32, device=cuda))
+    items = plan.mem[:8].view(torch.int32)[1].item()  # the split begins with its tag and its number of items
+    assert n <= items <= 2048 + n

@@ -354,7 +354,9 @@ __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__
         if (lane_id() == 63) many[k][tid >> 6] = mine[k];
     }
     __syncthreads();
-    uint32_t S = max((total + fine - 1) / fine, 1u);
+    // (a total that was cut off, of sequences that share most of their blocks, would give more items than there is room
+    // for: each sequence gets one)
+    uint32_t S = total < kMaxRows ? max((total + fine - 1) / fine, 1u) : 1u << 24;
 #pragma unroll
     for (int k = 2; k >= 0; k--) {
         uint32_t m = 0;
