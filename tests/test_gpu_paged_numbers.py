@@ -198,3 +198,17 @@ def test_plan_of_more_units_than_a_sum_holds(cuda):
     plan.update(ids=torch.zeros(n, dtype=torch.int32, device=cuda))
     items = plan.mem[:8].view(torch.int32)[1].item()  # the split begins with its tag and its number of items
     assert n <= items <= 2048 + n
+
+
+def test_a_step_with_room_for_every_row(cuda):
+    """Row buffers of 2^31 - 1 rows: the last ones are written too."""
+    rows = 2 ** 31 - 1
+    t = P.PagedTable.create(2, 4, 8, 16, device=cuda)
+    positions, slots = (torch.full((rows,), 77, dtype=torch.int32, device=cuda) for _ in range(2))
+    start, status = ints([7, 7, 7], cuda), ints([7, 7], cuda)
+    t.extend(ints([3, 20], cuda), start, positions, slots, status)
+    assert start.tolist() == [0, 3, 23] and status.tolist() == [0, 0]
+    assert positions[:24].tolist() == [0, 1, 2, *range(20), 0]
+    assert slots[:23].tolist() == [0, 1, 2, *range(16, 36)]
+    for at in range(23, rows, 2 ** 28):
+        assert bool((positions[at:at + 2 ** 28] == 0).all()) and bool((slots[at:at + 2 ** 28] == -1).all())

@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(kRowsPerGroup) rows_kernel(TableArgs t, const 
     extern __shared__ uint32_t start[];
     for (int i = threadIdx.x; i <= n; i += kRowsPerGroup) start[i] = uint32_t(start_in[i]);
     __syncthreads();
+    if (blockIdx.x * kRowsPerGroup + threadIdx.x >= uint32_t(max_rows)) return;
     const int r = blockIdx.x * kRowsPerGroup + threadIdx.x;
-    if (r >= max_rows) return;
     int pos = 0, slot = -1;
     if (uint32_t(r) < start[n]) {
         const int i = find(start, n, uint32_t(r)), st = status[i];
@@ -498,7 +498,7 @@ extern "C" int vireo_paged_extend(const vireo_paged_table *t, const int32_t *ids
                            positions, slots, status, here);
     }
     if (!here)
-        hipLaunchKernelGGL(rows_kernel, dim3((max_rows + kRowsPerGroup - 1) / kRowsPerGroup), dim3(kRowsPerGroup),
+        hipLaunchKernelGGL(rows_kernel, dim3((uint32_t(max_rows) + kRowsPerGroup - 1) / kRowsPerGroup), dim3(kRowsPerGroup),
                            4 * size_t(n + 1), s, a, ids, n, max_rows, start, status, positions, slots);
     return vh_finish(s, vh_check(hipGetLastError()));
 }
