@@ -137,7 +137,8 @@ typedef struct {
  * neither the cache nor q_out changes. Two rows of one call must not have the
  * same slot. With c->means, a row in the last slot of a block also sets that
  * block's mean key, from the keys as stored; those of the block's other slots
- * have to be there by the end of the call. */
+ * have to be there by the end of the call. -E2BIG for more heads of rows than one
+ * launch takes (2^28 queries and keys of 256, 2^30 of 64, or somewhat fewer beside the values). */
 int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_rows *r, void *stream);
 
 /* ---- attention of one new token per sequence ------------------------------------ */

@@ -176,3 +176,13 @@ def test_queries_in_place_keep_their_rows(lib, kw):
 def test_attention_in_place_keeps_its_rows(lib):
     t = table()
     assert lib.vireo_paged_attend(C.byref(cache()), C.byref(plan(t)), PTR, 30, 1024, 1.0, None, PTR, 2048, None) == BAD
+
+
+@pytest.mark.parametrize("hs,n_rows,n_heads", [(128, 2 ** 26, 8), (256, 2 ** 24, 30), (64, 2 ** 28, 8), (64, 2 ** 30, 1),
+                                               (64, 2 ** 31 - 1, 65535)])
+def test_more_rows_than_a_launch_takes(lib, hs, n_rows, n_heads):
+    """Refused before any device work: 2^32 threads and more, 256 / (hs / 16) head rows to 256 of them."""
+    c = cache(head_size=hs)
+    r = rows(rows=n_rows, n_heads=n_heads, rotary=0, q_stride=n_heads * hs, k_stride=2 * hs, v_stride=2 * hs,
+             q_out_stride=n_heads * hs)
+    assert lib.vireo_paged_append(C.byref(c), C.byref(r), None) == -errno.E2BIG

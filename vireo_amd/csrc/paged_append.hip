@@ -188,16 +188,18 @@ __global__ void __launch_bounds__(256) means_kernel(const int32_t *__restrict__ 
 }
 
 template <int HS>
-void launch_append(AppendArgs a, uint16_t *means, hipStream_t s) {
+int launch_append(AppendArgs a, uint16_t *means, hipStream_t s) {
     const vireo_paged_rows &r = a.r;
     constexpr int kGroups = 256 / (HS / 16);  // head rows of a workgroup
-    const int64_t heads = int64_t(r.rows) * (r.n_heads + a.n_kv);
-    const int64_t values = int64_t((r.rows + kVRows - 1) / kVRows) * a.n_kv;
-    a.qk_groups = int((heads + kGroups - 1) / kGroups);
-    hipLaunchKernelGGL(append_kernel<HS>, dim3(unsigned(a.qk_groups + values)), dim3(256), 0, s, a);
+    const int64_t heads = int64_t(r.rows) * (r.n_heads + a.n_kv), qk = (heads + kGroups - 1) / kGroups;
+    const int64_t values = (int64_t(r.rows) + kVRows - 1) / kVRows * a.n_kv;
+    if ((qk + values) * 256 >= int64_t(1) << 32) return -E2BIG;  // threads of a launch
+    a.qk_groups = int(qk);
+    hipLaunchKernelGGL(append_kernel<HS>, dim3(unsigned(qk + values)), dim3(256), 0, s, a);
     if (means)
         hipLaunchKernelGGL(means_kernel<HS>, dim3((r.rows + kMeanRows - 1) / kMeanRows, a.n_kv), dim3(256), 0, s,
                            r.slots, r.rows, a.slots, a.shift, a.n_kv, a.cache_type, a.k, means);
+    return vh_check(hipGetLastError());
 }
 
 }  // namespace
@@ -216,15 +218,13 @@ extern "C" int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_
         r->rotary < 0 || r->rotary % 16 || r->rotary > hs || (r->rotary > 0 && (!r->rope || r->max_pos < 1)) ||
         !(r->eps >= 0.0f))
         return -EINVAL;
-    const int64_t heads = int64_t(r->rows) * (r->n_heads + 2 * int64_t(c->n_kv_heads));
-    if (heads > (int64_t(1) << 31)) return -E2BIG;
     int shift = 4;
     while ((1 << shift) < c->block_tokens) shift++;
     const AppendArgs a{*r, static_cast<uint16_t *>(c->k), static_cast<uint16_t *>(c->v), c->type, c->n_kv_heads, shift,
                  c->n_blocks * c->block_tokens, 0};
     uint16_t *means = static_cast<uint16_t *>(c->means);
-    if (hs == 64) launch_append<64>(a, means, s);
-    else if (hs == 128) launch_append<128>(a, means, s);
-    else launch_append<256>(a, means, s);
-    return vh_finish(s, vh_check(hipGetLastError()));
+    const int rc = hs == 64    ? launch_append<64>(a, means, s)
+                   : hs == 128 ? launch_append<128>(a, means, s)
+                               : launch_append<256>(a, means, s);
+    return rc == -E2BIG ? rc : vh_finish(s, rc);
 }
