@@ -212,3 +212,26 @@ def test_a_step_with_room_for_every_row(cuda):
     assert slots[:23].tolist() == [0, 1, 2, *range(16, 36)]
     for at in range(23, rows, 2 ** 28):
         assert bool((positions[at:at + 2 ** 28] == 0).all()) and bool((slots[at:at + 2 ** 28] == -1).all())
+
+
+def test_the_most_sequences_and_heads(cuda):
+    """4 096 sequences of 4 096 heads, all empty but the last, which is split and joined by the second launch."""
+    n, H, d, G, t = 4096, 4096, 64, 16, 5000
+    nb = -(-t // G)
+    blocks = torch.zeros((n, nb), dtype=torch.int32, device=cuda)
+    blocks[n - 1] = torch.arange(nb, dtype=torch.int32, device=cuda)
+    length = torch.zeros(n, dtype=torch.int32, device=cuda)
+    length[n - 1] = t
+    table = P.PagedTable(blocks, length, torch.zeros(nb, dtype=torch.int32, device=cuda), ints([0], cuda), G)
+    k, v = randn((nb, 1, G, d), BF, cuda, 41), randn((nb, 1, d, G), BF, cuda, 42)
+    cache = P.PagedCache(k, v)
+    plan = P.PagedPlan(table, cache, n, H)
+    plan.update()
+    q = torch.zeros((n, H, d), dtype=BF, device=cuda)
+    q[n - 1] = randn((H, d), BF, cuda, 43)
+    out = torch.full_like(q, 7.0)
+    cache.attend(q, out, plan)
+    assert not bool(out[:n - 1].any())
+    ref, weight, size = attend64(q[n - 1], k[:, 0], v[:, 0], list(range(nb)), [min(G, t - x * G) for x in range(nb)], 0.125)
+    err = (out[n - 1].double() - ref).abs()
+    assert bool((err <= half_step(BF) * ref.abs() + working(weight, size, d)).all())

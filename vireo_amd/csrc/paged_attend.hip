@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendArgs a) {
     constexpr int ND = D / 4, NG = 256 / ND, U = 8;
     __shared__ f32x4 red[NG][ND];
     __shared__ float fs[256], wm[4], wl[4];
-    const int seq = blockIdx.x / a.n_heads, h = blockIdx.x - seq * a.n_heads;
+    const int seq = blockIdx.y, h = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const uint32_t tag = a.head->tag;
     const int f0 = a.first[seq], n = a.first[seq + 1] - f0;
@@ -515,7 +515,7 @@ void launch_attend(const AttendArgs &a, int cap, int n, hipStream_t s) {
     const dim3 grid(a.n_kv * a.tiles, cap);
     if (a.shift < 6) hipLaunchKernelGGL((attend_kernel<D, T, QF, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attend_kernel<D, T, QF, false>), grid, dim3(256), 0, s, a);
-    if (!a.arrivals) hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(unsigned(n) * a.n_heads), dim3(256), 0, s, a);
+    if (!a.arrivals) hipLaunchKernelGGL((merge_kernel<D, T, QF>), dim3(a.n_heads, n), dim3(256), 0, s, a);
 }
 
 template <int D>
