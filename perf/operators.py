@@ -374,10 +374,13 @@ _stream = None
 
 
 def _serving_stream():
-    """The stream that the program serves on (calls on the default stream are synchronous)."""
+    """The stream that the program serves on (calls on the default stream are synchronous). It becomes the current one
+    with the first pass: after the inputs that were made before, and before whatever is done with outputs later."""
     global _stream
     if _stream is None:
         _stream = torch.cuda.Stream()
+        _stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(_stream)
     return _stream
 
 
