@@ -12,10 +12,15 @@
             cache.attend(q_out, out, plan)
 
 As with every call of the library, a call on the default stream waits for its
-work; on a stream (the current one, or `stream=`) it is only enqueued. Every
-tensor must be on the table's or cache's device, which need not be the current
-one. Arguments that the library would misread raise ValueError here; what it
-refuses itself raises VireoError.
+work; on a stream (the current one, or `stream=`) it is only enqueued. Where
+`stream=` is not the current one, the call's tensors are recorded on it, so that
+they may be dropped before its work is done (tensors made on the current stream
+need nothing, as with torch's own calls); that inputs are there when it begins
+and that outputs are read after it is the caller's to order, and so is that the
+tensors of a captured graph live as long as it. Every tensor must be on the
+table's or cache's device, which need not be the current one. Arguments that the
+library would misread raise ValueError here; what it refuses itself raises
+VireoError.
 """
 import ctypes as C
 import math
@@ -68,12 +73,23 @@ class _On:
         self.index = device.index
         self.alone = torch.cuda.device_count() == 1
 
-    def call(self, name, stream, *args):
+    def call(self, name, stream, tensors, handles, *args):
+        """tensors: the call's (or None); handles: the objects whose own tensors it uses."""
         fn = getattr(self.lib, name)
         if stream is None:
             stream = torch.cuda.current_stream(self.device)
         elif stream.device_index != self.index:
             raise ValueError(f"a stream of {self.device} is needed")
+        elif torch.accelerator.current_stream(self.index).stream_id != stream.stream_id:
+            # the tensors' memory is not to be given to others before this stream's work is done (0.3 us each)
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+            for h in handles:
+                if stream.cuda_stream not in h.streams:
+                    h.streams.add(stream.cuda_stream)
+                    for t in h.own:
+                        t.record_stream(stream)
         if self.alone or torch.cuda.current_device() == self.index:
             rc = fn(*args, stream.cuda_stream)
         else:
@@ -102,6 +118,7 @@ class PagedTable:
                                   _ints(free_blocks, free_blocks.shape, dev, "free_blocks"),
                                   _ints(n_free, (1,), dev, "n_free"))
         self._p = C.pointer(self.c)
+        self.own, self.streams = (blocks, length, free_blocks, n_free), set()
 
     @classmethod
     def create(cls, max_seqs, max_blocks, n_blocks, block_tokens, device="cuda", stream=None):
@@ -117,7 +134,7 @@ class PagedTable:
         return t
 
     def reset(self, stream=None):
-        self.on.call("vireo_paged_reset", stream, self._p)
+        self.on.call("vireo_paged_reset", stream, (), (self,), self._p)
 
     def _ids(self, ids, n):
         if ids is None:
@@ -129,8 +146,8 @@ class PagedTable:
         0 .. n - 1): fills start [n + 1], positions and slots [max_rows] and status
         [n] (0 or a negative errno, per sequence: see the header)."""
         n, rows, dev = status.numel(), slots.numel(), self.index
-        self.on.call("vireo_paged_extend", stream, self._p, self._ids(ids, n),
-                     None if n_new is None else _ints(n_new, (n,), dev, "n_new"), n, rows,
+        self.on.call("vireo_paged_extend", stream, (ids, n_new, start, positions, slots, status), (self,), self._p,
+                     self._ids(ids, n), None if n_new is None else _ints(n_new, (n,), dev, "n_new"), n, rows,
                      _ints(start, (n + 1,), dev, "start"), _ints(positions, (rows,), dev, "positions"),
                      _ints(slots, (rows,), dev, "slots"), _ints(status, (n,), dev, "status"))
 
@@ -138,7 +155,7 @@ class PagedTable:
         """Sequences ids cut back to new_len tokens (None: to none, which ends them);
         ids None: as many as new_len has, or every sequence."""
         n = ids.numel() if ids is not None else new_len.numel() if new_len is not None else self.max_seqs
-        self.on.call("vireo_paged_truncate", stream, self._p, self._ids(ids, n),
+        self.on.call("vireo_paged_truncate", stream, (ids, new_len), (self,), self._p, self._ids(ids, n),
                      None if new_len is None else _ints(new_len, (n,), self.index, "new_len"), n)
 
 
@@ -151,7 +168,7 @@ class PagedPlan:
     def __init__(self, table, cache, n, n_heads, list_blocks=0):
         self.table, self.n, self.n_heads, self.list_blocks = table, n, n_heads, list_blocks
         self.n_kv_heads, self.head_size = cache.n_kv_heads, cache.head_size
-        self.ids = None
+        self.ids = None  # of the last update
         self._shape = (n, n_heads, cache.head_size)
         self._lists = (n, cache.n_kv_heads, list_blocks)
         self.index = table.index
@@ -162,14 +179,15 @@ class PagedPlan:
             _lib.check(int(nbytes), "vireo_paged_plan_bytes")
         self.mem = torch.zeros(int(nbytes), dtype=torch.uint8, device=table.device)
         self.c.mem = self.mem.data_ptr()
+        self.own, self.streams = (self.mem,), set()
         # zeroed on the current stream; the plan may serve on another
         torch.cuda.current_stream(table.device).synchronize()
 
     def update(self, ids=None, stream=None):
         """By the table's lengths now; ids [n]: the batch's sequences (None: 0 .. n - 1)."""
         self.c.ids = self.table._ids(ids, self.n)
-        self.ids = ids  # the update, or a graph that holds it, reads it later
-        self.table.on.call("vireo_paged_plan_update", stream, self._p)
+        self.ids = ids
+        self.table.on.call("vireo_paged_plan_update", stream, (ids,), (self, self.table), self._p)
 
 
 class PagedCache:
@@ -192,6 +210,7 @@ class PagedCache:
         self.c = _lib.PagedCacheC(_TYPES[k.dtype], nb, G, kv, d, k.data_ptr(), v.data_ptr(),
                                   None if means is None else means.data_ptr())
         self._p = C.pointer(self.c)
+        self.own, self.streams = (k, v) if means is None else (k, v, means), set()
 
     @classmethod
     def create(cls, table, n_kv_heads, head_size, dtype=torch.bfloat16, means=False):
@@ -224,10 +243,13 @@ class PagedCache:
                             None if k_norm is None else _floats(k_norm, d, dev, "k_norm"), eps,
                             None if rope is None else _floats(rope, max_pos * rotary, dev, "rope"), rotary, max_pos,
                             _ints(positions, (T,), dev, "positions"), _ints(slots, (T,), dev, "slots"), op, ot, os_)
-        self.on.call("vireo_paged_append", stream, self._p, C.byref(r))
+        self.on.call("vireo_paged_append", stream,
+                     (q, k, v, positions, slots, q_out, rope, q_norm, k_norm, q_bias, k_bias, v_bias), (self,), self._p,
+                     C.byref(r))
 
     def _plan(self, plan):
-        _need(plan.index == self.index, f"a plan on {self.device} is needed")
+        if plan.index != self.index:
+            raise ValueError(f"a plan on {self.device} is needed")
         return plan._p
 
     def attend(self, q, out, plan, lists=None, scale=None, stream=None):
@@ -236,11 +258,13 @@ class PagedCache:
         list_blocks] of them; scale: 1 / sqrt(head_size) if None."""
         qp, qt, qs = _rows(q, plan._shape, self.index, "q")
         op, ot, os_ = _rows(out, plan._shape, self.index, "out")
-        _need(qt == ot, "q and out have to be of one type")
-        _need((lists is not None) == (plan.list_blocks > 0), "lists go with a plan for lists, and only with one")
+        if qt != ot:
+            raise ValueError("q and out have to be of one type")
+        if (lists is not None) != (plan.list_blocks > 0):
+            raise ValueError("lists go with a plan for lists, and only with one")
         lp = None if lists is None else _ints(lists, plan._lists, self.index, "lists")
-        self.on.call("vireo_paged_attend", stream, self._p, self._plan(plan), qp, qt, qs,
-                     1.0 / math.sqrt(self.head_size) if scale is None else scale, lp, op, os_)
+        self.on.call("vireo_paged_attend", stream, (q, out, lists), (self, plan, plan.table), self._p, self._plan(plan),
+                     qp, qt, qs, 1.0 / math.sqrt(self.head_size) if scale is None else scale, lp, op, os_)
 
     def select(self, q, plan, lists, sinks=0, window=1, stream=None):
         """lists [n, n_kv_heads, plan.list_blocks]: the first `sinks` blocks of each
@@ -248,4 +272,5 @@ class PagedCache:
         ascending order, -1 behind them."""
         qp, qt, qs = _rows(q, plan._shape, self.index, "q")
         lp = _ints(lists, plan._lists, self.index, "lists")
-        self.on.call("vireo_paged_select", stream, self._p, self._plan(plan), qp, qt, qs, sinks, window, lp)
+        self.on.call("vireo_paged_select", stream, (q, lists), (self, plan, plan.table), self._p, self._plan(plan),
+                     qp, qt, qs, sinks, window, lp)
