@@ -107,3 +107,23 @@ def test_a_handle_records_its_tensors_on_every_stream(cuda):
         torch.cuda.synchronize()
     for h in (plan, b.table, b.cache):
         assert h.streams == {s.cuda_stream for s in streams}
+
+
+def test_counts_past_32_bits_are_refused(cuda):
+    """A C int would hold their low bits, which are counts that the library takes."""
+    b = Batch(cuda, [100], 4, 2, 64, 16, BF, BF, seed=53)
+    more = 2 ** 32
+    with pytest.raises(ValueError):
+        P.PagedTable(b.table.blocks, b.table.len, b.table.free_blocks, b.table.n_free, more + 16)
+    for n, heads, lists in ((more + 1, 4, 0), (1, more + 4, 0), (1, 4, more)):
+        with pytest.raises(ValueError):
+            P.PagedPlan(b.table, b.cache, n, heads, lists)
+    cache = P.PagedCache(b.k, b.v, torch.zeros((b.cache.n_blocks, 2, 64), dtype=BF, device=cuda))
+    plan = P.PagedPlan(b.table, cache, 1, 4, 5)
+    plan.update(ids=b.tids)
+    lists = torch.zeros((1, 2, 5), dtype=torch.int32, device=cuda)
+    for sinks, window in ((more, 1), (1, more + 1), (-more, 1)):
+        with pytest.raises(ValueError):
+            cache.select(b.q, plan, lists, sinks=sinks, window=window)
+    cache.select(b.q, plan, lists, sinks=1, window=1)
+    assert lists[0, 0].tolist()[0] == 0

@@ -38,6 +38,13 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+def _count(v, name):
+    """v, which a C int would otherwise hold the low bits of."""
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{name}: a count within 32 bits is needed")
+    return v
+
+
 def _ints(t, shape, dev, name):
     """The address of a contiguous int32 tensor of this shape; dev: the device's index."""
     if t.dtype is not _I32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
@@ -110,7 +117,7 @@ class PagedTable:
         self.device = blocks.device
         self.index = dev = blocks.get_device()
         self.max_seqs, self.max_blocks = blocks.shape
-        self.n_blocks, self.block_tokens = free_blocks.numel(), block_tokens
+        self.n_blocks, self.block_tokens = free_blocks.numel(), _count(block_tokens, "block_tokens")
         self.blocks, self.len, self.free_blocks, self.n_free = blocks, length, free_blocks, n_free
         self.c = _lib.PagedTableC(self.max_seqs, self.max_blocks, self.n_blocks, block_tokens,
                                   _ints(blocks, blocks.shape, dev, "blocks"),
@@ -166,7 +173,8 @@ class PagedPlan:
     stream at a time."""
 
     def __init__(self, table, cache, n, n_heads, list_blocks=0):
-        self.table, self.n, self.n_heads, self.list_blocks = table, n, n_heads, list_blocks
+        self.table, self.n, self.n_heads = table, _count(n, "n"), _count(n_heads, "n_heads")
+        self.list_blocks = _count(list_blocks, "list_blocks")
         self.n_kv_heads, self.head_size = cache.n_kv_heads, cache.head_size
         self.ids = None  # of the last update
         self._shape = (n, n_heads, cache.head_size)
@@ -272,5 +280,7 @@ class PagedCache:
         ascending order, -1 behind them."""
         qp, qt, qs = _rows(q, plan._shape, self.index, "q")
         lp = _ints(lists, plan._lists, self.index, "lists")
+        if not (-2 ** 31 <= sinks < 2 ** 31 and -2 ** 31 <= window < 2 ** 31):
+            raise ValueError("sinks and window: counts within 32 bits are needed")
         self.on.call("vireo_paged_select", stream, (q, lists), (self, plan, plan.table), self._p, self._plan(plan),
                      qp, qt, qs, sinks, window, lp)
