@@ -235,3 +235,14 @@ def test_the_most_sequences_and_heads(cuda):
     ref, weight, size = attend64(q[n - 1], k[:, 0], v[:, 0], list(range(nb)), [min(G, t - x * G) for x in range(nb)], 0.125)
     err = (out[n - 1].double() - ref).abs()
     assert bool((err <= half_step(BF) * ref.abs() + working(weight, size, d)).all())
+
+
+@pytest.mark.parametrize("H,KV,cache,query", [(1, 1, BF, F32), (2, 2, HF, HF), (4, 1, BF, BF), (6, 2, HF, F32)])
+def test_joins_of_more_items_than_one_go_of_wide_heads(cuda, H, KV, cache, query):
+    """Up to 32 items of heads of 256, of which the last workgroup takes 16 at a time; alone and beside others."""
+    for lens in ([4096], [4000, 0, 1, 3001]):
+        b = Batch(cuda, lens, H, KV, 256, 64, cache, query, seed=44, spread=2.0)
+        b.table = P.PagedTable(b.table.blocks[:, :64].contiguous(), b.table.len, b.table.free_blocks, b.table.n_free, 64)
+        out = b.attend()
+        b.check(out)
+        assert torch.equal(out, b.attend())

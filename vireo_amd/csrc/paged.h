@@ -52,9 +52,12 @@ inline bool vh_in_place_ok(const void *from, uint32_t from_type, int64_t from_st
 // workgroup. Where the table or the lists leave a sequence few units, at most
 // kJoinUnits and kJoinHeads units and heads of a workgroup together, the last
 // workgroup of a sequence and kv head to finish joins its items (arrivals counts
-// them), else a second launch does. One sequence, 8 heads a kv head, 4 layers: 8
-// units 35.4 us joined and 44.5 in two launches, 16 units 40.7 and 46.7, 24 units 46.5 and
-// 46.7, 31 units 53.2 and 46.9 (of 16 heads 72.7 and 47.1).
+// them), else a second launch does. Per call, joined and in two launches: one sequence,
+// 8 heads of 128 a kv head 8 units 8.0 and 10.6 us, 16 units 9.2 and 10.7; 4 heads 8 units 8.1 and 10.4, 16
+// units 9.8 and 10.6, 24 units 11.7 and 10.6, 32 units 13.7 and 10.7; 4 of 256 32 units 16.3
+// and 13.5. 8 sequences, whose split gives each fewer items: 4 heads of 128 16 units 15.4 and
+// 16.8, 32 units 24.5 and 26.5. So the rule costs one sequence alone 1 to 3 us between 17 and 32
+// units and gains a batch 2. (In a graph the second launch costs 1 us less.)
 constexpr int kJoinUnits = 32, kJoinHeads = 128;
 struct PlanHead {
     uint32_t tag;  // written by an update of a plan of the same shape (vh_plan_tag)
