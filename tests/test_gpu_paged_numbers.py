@@ -246,3 +246,16 @@ def test_joins_of_more_items_than_one_go_of_wide_heads(cuda, H, KV, cache, query
         out = b.attend()
         b.check(out)
         assert torch.equal(out, b.attend())
+
+
+@pytest.mark.parametrize("G", [16, 128])
+@pytest.mark.parametrize("value", [3e38, 1e-39, -2.5e38])
+def test_means_of_the_largest_and_smallest_keys(cuda, G, value):
+    """A block's mean key where the sum of its keys is beyond fp32, and where keys are subnormal: equal keys' mean is the key."""
+    k, v = (torch.zeros(s, dtype=BF, device=cuda) for s in ((2, 1, G, 64), (2, 1, 64, G)))
+    means = torch.zeros((2, 1, 64), dtype=BF, device=cuda)
+    x = torch.full((G, 3, 64), value, dtype=BF, device=cuda)
+    rows = torch.arange(G, dtype=torch.int32, device=cuda)
+    P.PagedCache(k, v, means).append(x[:, :1], x[:, 1:2], x[:, 2:], rows, rows + G, torch.zeros_like(x[:, :1]))
+    assert bool((k[1] == x[0, 0, 0]).all()) and bool((means[1] == x[0, 0, 0]).all())
+    assert not bool(means[0].any())

@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(256) means_kernel(const int32_t *__restrict__ 
         if (slot < 0 || slot >= n_slots || (slot & (G - 1)) != G - 1) continue;
         const size_t head = size_t(slot >> shift) * n_kv + h;
         const uint16_t *src = k + (head * G + tok) * HS + 4 * sub;
+        const float share = 1.0f / float(G);  // a power of two: exact, and the sum does not leave fp32
         float sum[E] = {};
 #pragma unroll 4
         for (int g = 0; g < G; g += 4)
@@ -164,15 +165,14 @@ __global__ void __launch_bounds__(256) means_kernel(const int32_t *__restrict__ 
                 for (int j = 0; j < 2; j++) {
                     const float2 f = type == VIREO_PAGED_BF16 ? El<VIREO_PAGED_BF16>::unpack(w[j])
                                                               : El<VIREO_PAGED_F16>::unpack(w[j]);
-                    sum[e + 2 * j] += f.x;
-                    sum[e + 2 * j + 1] += f.y;
+                    sum[e + 2 * j] = fmaf(f.x, share, sum[e + 2 * j]);
+                    sum[e + 2 * j + 1] = fmaf(f.y, share, sum[e + 2 * j + 1]);
                 }
             }
 #pragma unroll
         for (int e = 0; e < E; e++) {
             sum[e] += __shfl_xor(sum[e], 16);
             sum[e] += __shfl_xor(sum[e], 32);
-            sum[e] *= 1.0f / float(G);  // a power of two: exact
         }
         if (tok == 0)
 #pragma unroll
