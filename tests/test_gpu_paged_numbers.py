@@ -259,3 +259,13 @@ def test_means_of_the_largest_and_smallest_keys(cuda, G, value):
     P.PagedCache(k, v, means).append(x[:, :1], x[:, 1:2], x[:, 2:], rows, rows + G, torch.zeros_like(x[:, :1]))
     assert bool((k[1] == x[0, 0, 0]).all()) and bool((means[1] == x[0, 0, 0]).all())
     assert not bool(means[0].any())
+
+
+@pytest.mark.parametrize("query", [BF, F32])
+@pytest.mark.parametrize("value", [3e38, -3.2e38])
+def test_the_largest_values(cuda, query, value):
+    """Values whose sum is beyond fp32: their mean is not."""
+    b = Batch(cuda, [2, 33, 300, 3000], 8, 2, 128, 16, BF, query, seed=45)
+    live = torch.isfinite(b.v) & (b.v.abs() < 100)
+    b.v.copy_(torch.where(live, torch.tensor(value, dtype=BF, device=cuda), b.v))
+    b.check(b.attend())

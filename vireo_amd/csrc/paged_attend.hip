@@ -40,7 +40,7 @@
 // largest, a weight at 2^-38 of the largest that its wave has seen. Infinite keys and
 // values meet parts that are 0, whose products are NaN: where a wave finds a NaN in its sums it
 // goes over its tiles again, with the least value of its sign in place of such parts of a query's
-// value (in every call that would be seen beside large keys), and with weights of 1 and 0.
+// value (in every call that would be seen beside large keys), and with weights that are all the same.
 //
 // Waves merge through LDS. A sequence of one item is then written; others' partial
 // results are joined in the items' order, so that the bits are the same every time:
@@ -230,9 +230,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             for (int d = 0; d < DT; d++) vv[d][j] &= keep;
         }
     };
-    // a weight, at most 1 (the difference before the scale: a large score's rounding would be an exponent); over fp16
-    // up to 2^14, so that the parts of small ones keep their bits
-    auto weight = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x - m, c, T == VIREO_PAGED_F16 ? 14.0f : 0.0f)); };
+    // a weight, the largest 2^up (the difference before the scale: a large score's rounding would be an exponent)
+    auto weight = [&](float x, float up) { return __builtin_amdgcn_exp2f(fmaf(x - m, c, up)); };
+    // fp16: so that the parts of small ones keep their bits; bf16: so that sums of the largest values stay in fp32
+    constexpr float kUp = T == VIREO_PAGED_F16 ? 14.0f : -24.0f;
     for (bool again = false;; again = true) {
         m = kLowest, l = 0.0f;
 #pragma unroll
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             float ps = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[j] = weight(x[j]);
+                x[j] = weight(x[j], kUp);
                 ps += x[j];
             }
             l = fmaf(l, cr, ps);
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
         if (!QF || again || !__any(l != l)) break;
     }
     // A NaN may be an infinite value's, under a weight of which a part is 0: what such values (and NaN) come to under
-    // weights of 1 and 0 takes its place. Rare, and looked for once: 8 to 32 comparisons a wave.
+    // weights that are all the same, or 0, takes its place. Rare, and looked for once: 8 to 32 comparisons a wave.
     bool odd = false;
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -317,8 +318,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             mask(w, x);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[j] = weight(x[j]);
-                x[j] = x[j] > 0.0f ? 1.0f : x[j];  // a NaN stays one
+                x[j] = weight(x[j], 0.0f);
+                x[j] = x[j] > 0.0f ? (T == VIREO_PAGED_F16 ? 1.0f : 0x1p-24f) : x[j];  // a NaN stays one
             }
             u32x4 pw;
 #pragma unroll
