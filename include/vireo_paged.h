@@ -53,7 +53,8 @@ enum { VIREO_PAGED_F32 = 0, VIREO_PAGED_F16 = 1, VIREO_PAGED_BF16 = 30 };
  * never write into its blocks). */
 typedef struct {
     int max_seqs;         /* sequences: 1 .. 4096 */
-    int max_blocks;       /* blocks a sequence may have */
+    int max_blocks;       /* blocks a sequence may have: no more than are needed (vireo_paged_select takes
+                             longer over wide tables, and vireo_paged_attend a second launch) */
     int n_blocks;         /* blocks of the pool; n_blocks * block_tokens < 2^31 */
     int block_tokens;     /* 16, 32, 64 or 128 */
     int32_t *blocks;      /* [max_seqs x max_blocks] */
@@ -117,7 +118,8 @@ typedef struct {
     const void *q, *k, *v;                  /* 16-byte aligned, and so are the rows */
     int64_t q_stride, k_stride, v_stride;   /* elements */
     const float *q_bias, *k_bias, *v_bias;  /* [heads x head_size], NULL: none */
-    const float *q_norm, *k_norm;           /* [head_size] RMSNorm weights of every head, NULL: no norm */
+    const float *q_norm, *k_norm;           /* [head_size] RMSNorm weights of every head, NULL: no norm (one over the
+                                               row's whole q or k goes before this call: vireo_rmsnorm) */
     float eps;
     const float *rope;                      /* [max_pos x rotary] from vireo_rope_table(base, rotary, max_pos) */
     int rotary;                             /* dimensions rotated, the first ones: a multiple of 16, <= head_size */
@@ -147,7 +149,11 @@ int vireo_paged_append(const vireo_paged_cache *c, const vireo_paged_rows *r, vo
  * (lengths change) and used by every layer. The fields describe the batch;
  * mem is device memory of vireo_paged_plan_bytes bytes, 256-byte aligned: the
  * split and the attention's partial results. Calls that may run at the same
- * time (other streams, graphs replayed at once) need plans of their own. */
+ * time (other streams, graphs replayed at once) need plans of their own. The
+ * memory says which shape it was split for (the fields but ids, and the table's
+ * max_seqs, max_blocks and block_tokens): where that is another, or there was no update
+ * yet, vireo_paged_attend and vireo_paged_select return 0 and leave out and lists as
+ * they were, since only the device knows. */
 typedef struct {
     const vireo_paged_table *table;
     const int32_t *ids;      /* [n] rows of the table, NULL: 0 .. n - 1; an id outside it is an empty sequence */
@@ -161,14 +167,19 @@ typedef struct {
 /* Bytes of plan memory, or -EINVAL. */
 int64_t vireo_paged_plan_bytes(const vireo_paged_plan *p);
 /* Split the batch by the lengths that the table has now. Before the first
- * attend of a step, after vireo_paged_extend. */
+ * attend or select of a step, after vireo_paged_extend. */
 int vireo_paged_plan_update(const vireo_paged_plan *p, void *stream);
 
 /* out_i = softmax(scale q_i . K) V over sequence i's tokens, its newest among
  * them (extend and append come first): q, out [n x n_heads x head_size], rows
  * q_stride / out_stride elements apart, of `type` (F32 or the cache's), 16-byte
- * aligned. out may be q, with its stride. scale > 0. An empty sequence gives zeros. Products, sums and the softmax
- * are in fp32 or exact: fp32 queries and the weights are split into three 16-bit parts.
+ * aligned. out may be q, with its stride. scale > 0. An empty sequence gives zeros.
+ * Products, sums and the softmax are in fp32 or exact: fp32 queries and the weights
+ * are split into three 16-bit parts (over fp16 what lies below 2^-38 of a head's
+ * largest query value or of the largest weight is cut off). There is one query per
+ * sequence, its newest token's: the tokens of a prompt, or of drafts, that need
+ * attention of their own go through extend, append and attend one by one (an id
+ * named twice attends to the same tokens twice).
  * lists (NULL unless p->list_blocks > 0): [n x n_kv_heads x list_blocks], for
  * each kv head the blocks of the sequence that its heads attend to, by their
  * number in the sequence; only a sequence's first min(its blocks, list_blocks)
@@ -187,7 +198,8 @@ int vireo_paged_attend(const vireo_paged_cache *c, const vireo_paged_plan *p, co
  * block first. A sequence of at most list_blocks blocks gets all of them, then
  * -1. c->means is required. -E2BIG for a table of more than 65536 blocks a sequence
  * beside sinks and window. Lengths are those at the plan's update. q as in
- * vireo_paged_attend. */
+ * vireo_paged_attend. Its time goes by the table's width too, not by the lengths alone,
+ * most of all beyond 8192 blocks a sequence. */
 int vireo_paged_select(const vireo_paged_cache *c, const vireo_paged_plan *p, const void *q, uint32_t type,
                        int64_t q_stride, int sinks, int window, int32_t *lists, void *stream);
 

@@ -23,9 +23,9 @@
 // soon as the scores are formed and values as soon as they are weighed, so a
 // wave has a tile of 64 hs bytes in flight nearly all the time. They are read
 // once, with the non-temporal hint: 64 sequences of 500 to 30 001 tokens (1.9 GB)
-// 343 -> 318 us, 6.1 TB/s - but for the values of blocks of 64 slots and more, whose lines
+// 343 -> 318 us (324 with what came later, 6.0 TB/s) - but for the values of blocks of 64 slots and more, whose lines
 // two tiles share (16 sequences, 275 MB: 78 us with the hint, 67 without; 60 in
-// blocks of 16 and 32). Bound by that read; the matrix cores are busy for 6 % of the
+// blocks of 16 and 32). Bound by that read; the matrix cores are busy for 8 % of the
 // time for the 64 sequences (16-bit queries).
 //
 // Precision: products of 16-bit parts are exact in the matrix cores and their

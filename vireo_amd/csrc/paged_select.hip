@@ -4,20 +4,21 @@
 //
 //   score_b = float32(max_h sum_j q_hj m_bj), the sum in fp64
 //
-// A sum of fp64 products of 16-bit and fp32 values is within 2^-50 of exact in
-// any order, so the fp32 score, and with it which of two blocks is higher, does
-// not depend on how the sum is split. (An fp32 sum would leave the order of
-// near blocks to the split.)
+// A sum of fp64 products of 16-bit and fp32 values is within 2^-45 of their sizes'
+// sum of exact in any order, so that the fp32 score, and with it which of two blocks is
+// higher, hangs on how the sum is split only where it lies that near to a border between two
+// fp32 values. (An fp32 sum would leave the order of near blocks to the split.)
 //
 // score_kernel: 16 lanes per mean key (16-bit, D / 16 consecutive values a
 // lane), four keys per group of 16 lanes; per query head the lanes' four sums are
 // transposed while they are reduced (5 exchanges instead of 16). 228 000 mean keys of
-// 128 (58 MB, 16 sequences of 9 000 to 65 536 tokens) against 4 heads each take 19.6 us
-// (24.2 with a block's kv heads far apart in the grid); against one head each 14.2,
-// which is the read; the rest is fp64. The fp64 matrix cores took 46.8, and
+// 128 (58 MB, 16 sequences of 9 000 to 65 536 tokens) against 4 heads each take 18.7 to
+// 19.2 us (19.6 beside 24.2 with a block's kv heads far apart in the grid); against one head each
+// 14.2, which is the read; the rest is fp64. The fp64 matrix cores took 46.8, and
 // 16-bit matrix products that leave only the heads near the highest to fp64 33.9.
-// choose_kernel: a workgroup per (sequence, kv head), its keys in registers,
-// finds the budget's lowest score by a histogram of 256 bins of their range and the
+// The grid is as wide as the table, whatever the lengths: workgroups behind a sequence's end return.
+// choose_kernel: a workgroup per (sequence, kv head), its keys in registers
+// (but for tables of more than 8 192 candidates, below), finds the budget's lowest score by a histogram of 256 bins of their range and the
 // ranks of the scores in its bin, and writes the blocks in order by one prefix sum.
 // Bound by its chain of loads, barriers and LDS atomics.
 #include <hip/hip_runtime.h>
@@ -134,8 +135,11 @@ constexpr uint32_t kFew = 64;
 constexpr int kMaxCandidates = 65536;
 
 // HELD: keys that a thread holds in registers (the host takes the fewest threads and
-// keys that hold every candidate). Straight code over them: a loop's keys from memory
-// or both forms of every pass took 7.4 us for 1 871 candidates, this 5.4.
+// keys that hold every candidate that the table has room for). Straight code over them: a loop's keys from memory
+// or both forms of every pass took 7.4 us for 1 871 candidates, this 5.4. 64 keys of
+// 1024 threads do not fit the 128 registers of each and spill (396 words): one sequence of 30 001
+// tokens takes 9.9 us for scores and choice in tables of 65 536 tokens and 10.4 of 131 136, but 58.6 of
+// 262 144 (blocks of 16, 4 kv heads), 150 000 tokens 62.5.
 template <int NT, int HELD>
 __global__ void __launch_bounds__(NT) choose_kernel(SelectArgs a) {
     __shared__ uint32_t hist[2][256], wlo[NT / 64], whi[NT / 64];

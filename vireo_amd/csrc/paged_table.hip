@@ -15,8 +15,10 @@ namespace {
 
 constexpr int kThreads = 1024, kFewThreads = 256;  // a batch of at most kFewThreads takes so many: barriers of 4 waves
 // Rows that extend's one workgroup numbers itself, four per thread at a time; more
-// take a second launch over the chip (193 sequences, 4 558 rows: 4.5 and 6.3 us in two
-// launches, 7.9 in one).
+// take a second launch over the chip. 193 sequences, 4 558 rows: kernels of 4.5 and 3.7 us in
+// two launches, 7.9 in one. 64 sequences, replayed in a graph: 4 096 rows 7.9 us in two and 7.5 in
+// one, 8 192 rows 8.4 and 10.9, 16 384 rows 9.5 and 18.7; called one by one the second launch
+// costs the host 3 us more.
 constexpr int kRowsHere = 8192;
 constexpr uint32_t kMaxRows = 0x7fffffff;
 
@@ -302,10 +304,11 @@ __global__ void __launch_bounds__(NT) truncate_kernel(TableArgs t, const int32_t
 // the batch's units / `whole`, or up to an eighth more, if the items then number
 // at most `whole`: each CU has one, and they end together. Sequences that do not
 // divide so (short ones beside long ones) are cut finer, S = units / `fine`, so that
-// workgroups that end early take up others: 131 071 tokens alone 111 us (2 layers)
-// whole and 136 fine, 16 equal sequences 79 and 84; 64 sequences of 500 to 30 001
-// tokens 408 and 353, 23 of 1 to 8 191 67 and 59. Between the two, 131 071 tokens take 113 at
-// 512, 121 at 1 024 and 162 at 4 096 workgroups, the 64 sequences 396, 364 and 354.
+// workgroups that end early take up others: 131 071 tokens alone 98 us (2 layers)
+// whole and 125 fine; 64 sequences of 500 to 30 001 tokens 465 to 490 and 329, 23 of 1 to
+// 8 191 67 and 54 (2 layers). With the first kernels 16 equal sequences took 79 and 84, and between
+// the two 131 071 tokens 113 at 512, 121 at 1 024 and 162 at 4 096 workgroups (111 whole), the 64
+// sequences 396, 364 and 354 (353 fine).
 // LDS: items' prefix sums [n + 1], tokens [n], rows [n].
 template <int NT>
 __global__ void __launch_bounds__(NT) plan_kernel(TableArgs t, const int32_t *__restrict__ ids, int n, int whole,
