@@ -169,7 +169,8 @@ class PagedTable:
 class PagedPlan:
     """The split of a batch's attention over the device, for n sequences of
     `table` and caches shaped like `cache`; list_blocks > 0: over lists of that
-    many blocks (PagedCache.select). update() once per step; its memory serves one
+    many blocks (PagedCache.select). update() once per step: before the first one
+    attend and select leave their outputs as they were. Its memory serves one
     stream at a time."""
 
     def __init__(self, table, cache, n, n_heads, list_blocks=0):
@@ -261,8 +262,8 @@ class PagedCache:
         return plan._p
 
     def attend(self, q, out, plan, lists=None, scale=None, stream=None):
-        """out [n, n_heads, head_size] = attention of q (one new token per sequence of
-        the plan) over the sequences' blocks, or over lists [n, n_kv_heads,
+        """out [n, n_heads, head_size] = attention of q (each sequence's newest token; of
+        a prompt appended at once only the last can be attended) over the sequences' blocks, or over lists [n, n_kv_heads,
         list_blocks] of them; scale: 1 / sqrt(head_size) if None."""
         qp, qt, qs = _rows(q, plan._shape, self.index, "q")
         op, ot, os_ = _rows(out, plan._shape, self.index, "out")
