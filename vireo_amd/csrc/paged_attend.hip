@@ -32,15 +32,16 @@
 // sums fp32 (fp16 values below 2^-14 are not flushed, but their products are added
 // as if they were that large: absolute errors of 2^-38 of the largest weight). An fp32
 // query is the sum of three truncated 16-bit parts (under a power of two per
-// head: Queries), and so is a weight, whatever the result's type: a result is rounded once. (Two
-// parts hold 16 bits of a weight in bf16; truncated, they took some results past a
-// border between two bf16 values. The third part's products cost nothing beside the read: 64 sequences 329.4 us with
-// two and 328.4 with three, 131 071 tokens alone 97.2 and 97.4.) The sum of weights is
-// of the fp32 values. Over fp16 a query's value is cut off at 2^-38 of the head's
-// largest, a weight at 2^-38 of the largest that its wave has seen. Infinite keys and
-// values meet parts that are 0, whose products are NaN: where a wave finds a NaN in its sums it
-// goes over its tiles again, with the least value of its sign in place of such parts of a query's
-// value (in every call that would be seen beside large keys), and with weights that are all the same.
+// head: Queries), and so is a weight, whatever the result's type: a result is rounded
+// once. (Two parts hold 16 bits of a weight in bf16; truncated, they took some results
+// past a border between two bf16 values. The third part's products cost nothing beside
+// the read: 64 sequences 329.4 us with two and 328.4 with three, 131 071 tokens alone
+// 97.2 and 97.4.) The sum of weights is of the fp32 values. Over fp16 a query's value is
+// cut off at 2^-38 of the head's largest, a weight at 2^-38 of the largest that its wave
+// has seen. Infinite keys and values meet parts that are 0, whose products are NaN:
+// where a wave finds a NaN in its sums it goes over its tiles again, with the least
+// value of its sign in place of such parts of a query's value (in every call that would
+// be seen beside large keys), and with weights that are all the same.
 //
 // Waves merge through LDS. A sequence of one item is then written; others' partial
 // results are joined in the items' order, so that the bits are the same every time:
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_kernel(AttendArg
             e = query.template parts<false>(qw);
         }
         // Neither 0, which would make a NaN of a slot's -inf, nor infinite. Products with the queries are below 2^40 where
-        // scale 2^-e lies under 2^-126: all weights are 1 either way.
+        // scale 2^-e lies under 2^-126: all weights are the same either way.
         two = ldexpf(1.0f, min(max(a.expo - e, -126), 126)), c = a.mant * two;
         for (int i = i0; i < i1; i++) {
             float x[8];
